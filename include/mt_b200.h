@@ -350,6 +350,42 @@ MT_API int mt_fused_ce_bwd(const void* hidden, const void* weight, const void* l
                            void* stream);
 
 /* ---------------------------------------------------------------------
+ * 8-bit rows: RMSNorm (with the residual add) and plain quantisation to int8
+ *   with one fp32 scale per row.  Inference only.  No counterpart in the
+ *   reference (bf16 projections).
+ *     s = round(hidden + residual)  [residual NULL: s = hidden]
+ *     v = s * w,  a = max |v|,  q = rint(v * (127 / a)),
+ *     scale = a / 127 * rsqrt(mean(s^2) + eps)
+ * so q * scale approximates RMSNorm(s) * w to half a step, a / 254 * rstd.  q
+ * holds exactly these integers for any row, whatever the order of the sum of
+ * squares.  A row whose a is below 2^-119 gives q = 0 and scale = 0; a row that
+ * holds an infinity or a NaN gives a NaN scale.
+ * hidden: [rows, dim] in act_dtype; residual / new_residual: [rows, dim] in
+ * res_dtype (act_dtype or MT_F32; new_residual may be residual itself);
+ * w: [dim] in MT_F32 or act_dtype; q: [rows, dim]; scale: [rows]; all
+ * contiguous, dim <= 32768.
+ * mt_quantize_rows_int8: the same with v = x and no norm (scale = a / 127).
+ * ------------------------------------------------------------------- */
+MT_API int mt_rms_norm_int8(const void* hidden, int act_dtype, const void* residual, int res_dtype,
+                            const void* w, int w_dtype, void* new_residual, int8_t* q,
+                            float* scale, int64_t rows, int64_t dim, float eps, void* stream);
+MT_API int mt_quantize_rows_int8(const void* x, int dtype, int8_t* q, float* scale, int64_t rows,
+                                 int64_t dim, void* stream);
+
+/* ---------------------------------------------------------------------
+ * 8-bit matrix product   y[m, n] = round((sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n])
+ *   tcgen05 kind::i8 (few tokens: dp4a).  No counterpart in the reference.
+ * x: [M, K], w: [N, K] int8 row-major, 16-byte aligned, K a multiple of 16 and
+ * below 131,072 (the int32 sum cannot overflow); x_scale: [M], w_scale: [N]
+ * fp32 (w_scale 16-byte aligned); out: [M, N] row-major in out_dtype, any
+ * alignment and any N (rows whose stride and base are multiples of 16 bytes
+ * leave through TMA).
+ * ------------------------------------------------------------------- */
+MT_API int mt_int8_gemm(const int8_t* x, const float* x_scale, const int8_t* w,
+                        const float* w_scale, void* out, int out_dtype, int64_t M, int64_t N,
+                        int64_t K, uint32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------
  * Fused AdamW with 16-bit weight copies   replaces torch.optim.AdamW(fused=True)
  *   (src/mega_trading/trainer.py:535-545) plus the per-forward bf16 weight
  *   casts of the reference's autocast (trainer.py:336); no counterpart kernel

@@ -91,6 +91,12 @@ PROTOTYPES: dict[str, tuple[object, list[object]]] = {
          c_i64p, c_i64p, c_i64p, c_i64p, c_i64p, c_i64p, c_i64p, c_float, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp,
          c_vp],
     ),
+    "mt_rms_norm_int8": (
+        c_int,
+        [c_vp, c_int, c_vp, c_int, c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_float, c_vp],
+    ),
+    "mt_quantize_rows_int8": (c_int, [c_vp, c_int, c_vp, c_vp, c_i64, c_i64, c_vp]),
+    "mt_int8_gemm": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp]),
     "mt_fused_ce_workspace_bytes": (c_i64, [c_i64, c_i64]),
     "mt_fused_ce_fwd": (
         c_int,
@@ -186,7 +192,7 @@ def read_status(device: torch.device) -> int:
 
 # kernel ids of the status word's high half (the kKernelId constants in csrc/)
 KERNEL_NAMES = {1: "attention forward", 2: "attention backward", 3: "fused cross-entropy", 4: "fused cross-entropy",
-                6: "projection GEMM", 15: "wait probe"}
+                6: "projection GEMM", 9: "8-bit matrix product", 15: "wait probe"}
 
 
 def describe_status(code: int) -> str:

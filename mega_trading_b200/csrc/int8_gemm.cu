@@ -1,0 +1,173 @@
+// 8-bit matrix product with a scale per token and per channel:
+//   y[m, n] = round( (sum_k x[m, k] w[n, k]) * xs[m] * ws[n] )
+// x [M, K] and w [N, K] int8 row-major, the sum exact in int32 (K < 131,072
+// keeps 128 * 128 * K below 2^31), the scales applied in fp32, one rounding to
+// the output type.  No counterpart in the reference (bf16 projections).
+//
+// Many tokens: the tcgen05 product of tile_gemm.cuh with kind::i8 (twice the
+// rate of 16-bit operands), scales in the epilogue.  Few tokens (M <= 16): the
+// product is bound by reading w once and by latency, and a 128-row MMA tile
+// would be almost empty, so a dot-product kernel reads w straight into
+// registers (16 bytes per lane, 8 lanes per channel) and multiplies with dp4a.
+#include "tile_gemm.cuh"
+
+namespace mt {
+namespace {
+
+constexpr uint32_t kKernelId = 9;
+constexpr int kMaxK = 131056;
+constexpr int kFewTokens = 16;
+
+template <typename TO>
+struct Int8Epilogue {
+  static constexpr uint32_t kKernelId = mt::kKernelId;
+  static constexpr int OUT_SIZE = sizeof(TO);
+  const float* xs;
+  const float* ws;
+  int n;
+  bool add, direct;
+
+  struct Row {
+    float xs;
+  };
+  __device__ __forceinline__ Row row(int m, bool live) const { return Row{live ? __ldg(xs + m) : 0.f}; }
+
+  __device__ __forceinline__ void pack(const uint32_t (&z)[32], const Row& r, int n0, uint32_t* words) const {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      float s[4];
+      if (n0 + j + 4 <= n) {
+        const float4 q = __ldg(reinterpret_cast<const float4*>(ws + n0 + j));  // n0 is a multiple of 32
+        s[0] = q.x; s[1] = q.y; s[2] = q.z; s[3] = q.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = n0 + j + e < n ? __ldg(ws + n0 + j + e) : 0.f;
+      }
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __int2float_rn((int)z[j + e]) * r.xs * s[e];
+      if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) words[j + e] = __float_as_uint(v[e]);
+      } else {
+        words[j / 2] = pack2<TO>(v[0], v[1]);
+        words[j / 2 + 1] = pack2<TO>(v[2], v[3]);
+      }
+    }
+  }
+};
+
+// 8 lanes per channel, 4 channels per warp; MT tokens (rows past M repeat the last one).
+template <typename TO, int MT>
+__global__ void __launch_bounds__(256) int8_few_kernel(const int8_t* __restrict__ x, const float* __restrict__ xs,
+                                                       const int8_t* __restrict__ w, const float* __restrict__ ws,
+                                                       TO* __restrict__ y, int M, int N, int K) {
+  const int sub = threadIdx.x & 7;
+  const int n = (blockIdx.x * 256 + threadIdx.x) >> 3;
+  const bool live = n < N;
+  const int8_t* wr = w + int64_t(live ? n : N - 1) * K;
+  int acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = 0;
+#pragma unroll 4
+  for (int k = sub * 16; k < K; k += 128) {
+    const int4 b = __ldg(reinterpret_cast<const int4*>(wr + k));
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int4 a = __ldg(reinterpret_cast<const int4*>(x + int64_t(min(m, M - 1)) * K + k));
+      acc[m] = __dp4a(a.x, b.x, acc[m]);
+      acc[m] = __dp4a(a.y, b.y, acc[m]);
+      acc[m] = __dp4a(a.z, b.z, acc[m]);
+      acc[m] = __dp4a(a.w, b.w, acc[m]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
+  if (!live) return;
+  const float s = ws[n];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    if ((m & 7) == sub && m < M) y[int64_t(m) * N + n] = from_f32<TO>(__int2float_rn(acc[m]) * xs[m] * s);
+}
+
+template <typename TO>
+int launch_few(const int8_t* x, const float* xs, const int8_t* w, const float* ws, TO* y, int M, int N, int K,
+               cudaStream_t s) {
+  const unsigned grid = (unsigned)((int64_t(N) * 8 + 255) / 256);
+  if (M == 1)
+    int8_few_kernel<TO, 1><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
+  else if (M == 2)
+    int8_few_kernel<TO, 2><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
+  else if (M <= 4)
+    int8_few_kernel<TO, 4><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
+  else if (M <= 8)
+    int8_few_kernel<TO, 8><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
+  else
+    int8_few_kernel<TO, 16><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
+  return check_launch("int8_gemm_few");
+}
+
+template <class C, typename TO>
+int launch_tiles(const int8_t* x, const float* xs, const int8_t* w, const float* ws, TO* y, int out_dtype, int M,
+                 int N, int K, uint32_t* status, cudaStream_t s) {
+  TileParams<Int8Epilogue<TO>> prm;
+  int st = tile_operand_map<C>(&prm.tm_a, x, false, M, K, K, 128);
+  if (st != MT_OK) return st;
+  if ((st = tile_operand_map<C>(&prm.tm_b, w, false, N, K, K, C::B_ROWS)) != MT_OK) return st;
+  const bool direct = (reinterpret_cast<uintptr_t>(y) & 15u) != 0 || (int64_t(N) * sizeof(TO)) % 16 != 0;
+  if (direct)
+    prm.tm_out = prm.tm_a;  // not used
+  else if ((st = tile_output_map(&prm.tm_out, y, out_dtype, M, N, N)) != MT_OK)
+    return st;
+  prm.M = M;
+  prm.N = N;
+  prm.n_k = (K + C::BK - 1) / C::BK;
+  prm.k_per_split = prm.n_k;
+  prm.split_rows = 0;
+  prm.out = y;
+  prm.ld_out = N;
+  prm.status = status;
+  prm.ep = Int8Epilogue<TO>{xs, ws, N, false, direct};
+  return launch_tile_gemm<C>(prm, 1, "int8_gemm", s);
+}
+
+template <typename TO>
+int run_int8(const int8_t* x, const float* xs, const int8_t* w, const float* ws, void* out, int out_dtype, int M,
+             int N, int K, uint32_t* status, cudaStream_t s) {
+  TO* y = static_cast<TO*>(out);
+  if (M <= kFewTokens) return launch_few<TO>(x, xs, w, ws, y, M, N, K, s);
+  // CTA pairs need enough 256 x 256 tiles to occupy most of the GPU; smaller
+  // products take 128 x 128 tiles, four times as many.
+  const int64_t pair_tiles = int64_t((M + 255) / 256) * ((N + 255) / 256);
+  if (pair_tiles >= get_sm_count() / 2)
+    return launch_tiles<TileCfg<kKindI8, false, false, 256, true>, TO>(x, xs, w, ws, y, out_dtype, M, N, K, status, s);
+  return launch_tiles<TileCfg<kKindI8, false, false, 128, false>, TO>(x, xs, w, ws, y, out_dtype, M, N, K, status, s);
+}
+
+}  // namespace
+}  // namespace mt
+
+using namespace mt;
+
+extern "C" int mt_int8_gemm(const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale, void* out,
+                            int out_dtype, int64_t M, int64_t N, int64_t K, uint32_t* status, void* stream) {
+  if (M < 0 || N <= 0 || K <= 0) return MT_ERR_INVALID_ARGUMENT;
+  if (out_dtype != MT_F32 && out_dtype != MT_F16 && out_dtype != MT_BF16) return MT_ERR_UNSUPPORTED_DTYPE;
+  if (M > 0x7fffffffLL - 256 || N > 0x7fffffffLL / 8 - 256 || K > kMaxK) return MT_ERR_INVALID_ARGUMENT;
+  if (K % 16 != 0) return MT_ERR_UNSUPPORTED_LAYOUT;  // 16-byte rows
+  if (M == 0) return MT_OK;
+  if (x_scale == nullptr || out == nullptr || status == nullptr) return MT_ERR_INVALID_ARGUMENT;
+  for (const void* q : {static_cast<const void*>(x), static_cast<const void*>(w), static_cast<const void*>(w_scale)})
+    if (q == nullptr || (reinterpret_cast<uintptr_t>(q) & 15u) != 0) return MT_ERR_UNSUPPORTED_LAYOUT;
+  int st = bind_device_of(x);
+  if (st != MT_OK) return st;
+  if ((st = check_arch()) != MT_OK) return st;
+  auto s = static_cast<cudaStream_t>(stream);
+  switch (out_dtype) {
+    case MT_F32: return run_int8<float>(x, x_scale, w, w_scale, out, out_dtype, (int)M, (int)N, (int)K, status, s);
+    case MT_F16: return run_int8<__half>(x, x_scale, w, w_scale, out, out_dtype, (int)M, (int)N, (int)K, status, s);
+    default: return run_int8<__nv_bfloat16>(x, x_scale, w, w_scale, out, out_dtype, (int)M, (int)N, (int)K, status, s);
+  }
+}

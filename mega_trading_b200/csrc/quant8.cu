@@ -1,0 +1,302 @@
+// 8-bit outputs with one scale per row: RMSNorm (with the residual add fused
+// in front) and plain row quantisation.  No counterpart in the reference,
+// which runs every projection in bf16; these feed mt_int8_gemm.
+//
+//   s = round(h + r)                      (ADD; else s = x)
+//   v_i = s_i * w_i                       (NORM; else v = s)
+//   a = max_i |v_i|,  q_i = rint(v_i * (127 / a)),  scale = a / 127 * rstd
+//   rstd = rsqrt(mean(s^2) + eps)         (NORM; else 1)
+//
+// The normalised row is rstd * v, so rstd cancels out of q: q depends on exact
+// products and an exact maximum only, never on the order in which the sum of
+// squares was taken, and is the same integer for any grouping of threads.  A
+// row whose a is below 2^-119 (127 / a would overflow) gives q = 0, scale = 0;
+// a row with an infinity or a NaN gives a NaN scale, so whatever is computed
+// from it is NaN too.
+//
+// Bound by HBM: each element is read once (plus the residual read and written)
+// and leaves as one byte.  The row stays in registers between the reduction
+// and the quantisation.  One warp owns a row of up to 1024 elements; wider
+// rows take 128, 256 or 1024 threads (their statistics meet in shared memory).
+// Accesses are 16-byte vectors when the width and every address allow it,
+// single elements (consecutive lanes on consecutive elements) otherwise.
+#include <cmath>
+
+#include "common.cuh"
+
+namespace mt {
+namespace {
+
+constexpr float kTinyAmax = 1.504632769052528e-36f;  // 2^-119
+constexpr int kMaxDim = 32768;
+
+template <typename T>
+__device__ __forceinline__ void load8f(const T* p, float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    load_vec<T, 8>(p, v);
+  } else {
+    float a[4], b[4];
+    load_vec<T, 4>(p, a);
+    load_vec<T, 4>(p + 4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = a[i];
+      v[i + 4] = b[i];
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8f(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    store_vec<T, 8>(p, v);
+  } else {
+    store_vec<T, 4>(p, {v[0], v[1], v[2], v[3]});
+    store_vec<T, 4>(p + 4, {v[4], v[5], v[6], v[7]});
+  }
+}
+
+// max that keeps a NaN of either side out (fmaxf) but lets the caller see it
+// through the sum of squares or the products' own propagation.
+struct QParams {
+  const void* x;
+  const void* res;   // ADD
+  const void* w;     // NORM
+  int w_f32;         // weight in fp32 (else in x's dtype)
+  void* new_res;     // ADD
+  int8_t* q;
+  float* scale;
+  int64_t rows;
+  int dim;
+  float eps;
+};
+
+enum { kPlain = 0, kNorm = 1, kAddNorm = 2 };
+
+// TPR threads own a row; each holds NC chunks of 8 elements.
+template <typename TX, typename TR, int MODE, int TPR, int NC, bool VEC>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quant8_kernel(const __grid_constant__ QParams p) {
+  constexpr int kBlock = TPR < 256 ? 256 : TPR;
+  constexpr int kRows = kBlock / TPR;
+  __shared__ float red[2][kBlock / 32];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / TPR;
+  const bool live = row < p.rows;
+  const int dim = p.dim;
+  const TX* x = static_cast<const TX*>(p.x) + row * dim;
+  const TR* r = static_cast<const TR*>(p.res) + row * dim;
+  TR* nr = static_cast<TR*>(p.new_res) + row * dim;
+  float v[NC][8];
+  float ss = 0.f;
+  // element e of chunk c: VEC 8 consecutive, else strided by the row's threads
+  auto col_of = [&](int c, int e) { return VEC ? (c * TPR + t) * 8 + e : (c * 8 + e) * TPR + t; };
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if constexpr (VEC) {
+      const int col = col_of(c, 0);
+      if (live && col < dim) {
+        load8f<TX>(x + col, v[c]);
+        if constexpr (MODE == kAddNorm) {
+          float rv[8];
+          load8f<TR>(r + col, rv);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[c][e] = round_to<TR>(v[c][e] + rv[e]);
+          store8f<TR>(nr + col, v[c]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int col = col_of(c, e);
+        v[c][e] = 0.f;
+        if (live && col < dim) {
+          v[c][e] = to_f32<TX>(x[col]);
+          if constexpr (MODE == kAddNorm) v[c][e] = round_to<TR>(v[c][e] + to_f32<TR>(r[col]));
+        }
+      }
+      if constexpr (MODE == kAddNorm) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (live && col_of(c, e) < dim) nr[col_of(c, e)] = from_f32<TR>(v[c][e]);
+      }
+    }
+  }
+  float amax = 0.f, bad = 0.f;  // bad: NaN once any product is NaN (fmaxf drops NaNs)
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if constexpr (MODE != kPlain) {
+      float wv[8];
+      if constexpr (VEC) {
+        const int col = col_of(c, 0);
+        if (col < dim) {
+          if (p.w_f32)
+            load8f<float>(static_cast<const float*>(p.w) + col, wv);
+          else
+            load8f<TX>(static_cast<const TX*>(p.w) + col, wv);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) wv[e] = 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int col = col_of(c, e);
+          wv[e] = 0.f;
+          if (col < dim)
+            wv[e] = p.w_f32 ? static_cast<const float*>(p.w)[col] : to_f32<TX>(static_cast<const TX*>(p.w)[col]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ss = fmaf(v[c][e], v[c][e], ss);
+        v[c][e] = __fmul_rn(v[c][e], wv[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      amax = fmaxf(amax, fabsf(v[c][e]));
+      bad = fmaf(v[c][e], 0.f, bad);  // 0, or NaN from an infinity or a NaN
+    }
+  }
+  ss = ss + bad;  // a non-finite product makes the row's statistics NaN
+  ss = warp_sum(ss);
+  amax = warp_max(amax);
+  if constexpr (TPR > 32) {
+    constexpr int kWarps = TPR / 32;
+    const int base = (threadIdx.x / TPR) * kWarps;
+    if (lane_id() == 0) {
+      red[0][warp_id()] = ss;
+      red[1][warp_id()] = amax;
+    }
+    __syncthreads();
+    ss = 0.f;
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      ss += red[0][base + i];
+      amax = fmaxf(amax, red[1][base + i]);
+    }
+  }
+  if (!live) return;
+  const bool some = amax >= kTinyAmax;
+  const float inv = some ? __fdiv_rn(127.f, amax) : 0.f;
+  if (t == 0) {
+    // plain rows: ss is 0, or NaN for a non-finite row
+    const float rs = MODE == kPlain ? 1.f + ss : rsqrtf(ss / float(dim) + p.eps);
+    p.scale[row] = some || isnan(ss) ? amax * rs / 127.f : 0.f;
+  }
+  int8_t* q = p.q + row * dim;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    int b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = __float2int_rn(__fmul_rn(v[c][e], inv));
+    if constexpr (VEC) {
+      const int col = col_of(c, 0);
+      if (col < dim) {
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lo |= (uint32_t(b[e]) & 0xFFu) << (8 * e);
+          hi |= (uint32_t(b[e + 4]) & 0xFFu) << (8 * e);
+        }
+        *reinterpret_cast<uint2*>(q + col) = make_uint2(lo, hi);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col_of(c, e) < dim) q[col_of(c, e)] = (int8_t)b[e];
+    }
+  }
+}
+
+bool al(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+template <typename TX, typename TR, int MODE, int TPR, int NC>
+int launch_q(const QParams& p, bool vec, cudaStream_t s) {
+  constexpr int kBlock = TPR < 256 ? 256 : TPR;
+  const int64_t grid = (p.rows + kBlock / TPR - 1) / (kBlock / TPR);
+  if (grid > 0x7fffffffLL) return MT_ERR_INVALID_ARGUMENT;
+  if (vec)
+    quant8_kernel<TX, TR, MODE, TPR, NC, true><<<(unsigned)grid, kBlock, 0, s>>>(p);
+  else
+    quant8_kernel<TX, TR, MODE, TPR, NC, false><<<(unsigned)grid, kBlock, 0, s>>>(p);
+  return check_launch(MODE == kPlain ? "quantize_rows_int8" : "rms_norm_int8");
+}
+
+template <typename TX, typename TR, int MODE>
+int dispatch(const QParams& p, cudaStream_t s) {
+  const bool vec = p.dim % 8 == 0 && al(p.x, 16) && al(p.q, 8) && (MODE == kPlain || al(p.w, 16)) &&
+                   (MODE != kAddNorm || (al(p.res, 16) && al(p.new_res, 16)));
+  const int chunks = (p.dim + 7) / 8;
+  if (chunks <= 32) return launch_q<TX, TR, MODE, 32, 1>(p, vec, s);
+  if (chunks <= 64) return launch_q<TX, TR, MODE, 32, 2>(p, vec, s);
+  if (chunks <= 96) return launch_q<TX, TR, MODE, 32, 3>(p, vec, s);
+  if (chunks <= 128) return launch_q<TX, TR, MODE, 32, 4>(p, vec, s);
+  if (chunks <= 256) return launch_q<TX, TR, MODE, 128, 2>(p, vec, s);
+  if (chunks <= 384) return launch_q<TX, TR, MODE, 128, 3>(p, vec, s);
+  if (chunks <= 512) return launch_q<TX, TR, MODE, 128, 4>(p, vec, s);
+  if (chunks <= 1024) return launch_q<TX, TR, MODE, 256, 4>(p, vec, s);
+  return launch_q<TX, TR, MODE, 1024, 4>(p, vec, s);
+}
+
+int check_shape(int64_t rows, int64_t dim) {
+  if (rows < 0 || dim <= 0) return MT_ERR_INVALID_ARGUMENT;
+  if (dim > kMaxDim) {
+    set_last_error_text("8-bit rows: dim must be at most 32768");
+    return MT_ERR_INVALID_ARGUMENT;
+  }
+  return MT_OK;
+}
+
+}  // namespace
+}  // namespace mt
+
+using namespace mt;
+
+extern "C" int mt_rms_norm_int8(const void* hidden, int act_dtype, const void* residual, int res_dtype, const void* w,
+                                int w_dtype, void* new_residual, int8_t* q, float* scale, int64_t rows, int64_t dim,
+                                float eps, void* stream) {
+  int st = check_shape(rows, dim);
+  if (st != MT_OK) return st;
+  const bool add = residual != nullptr;
+  if (w_dtype != MT_F32 && w_dtype != act_dtype) return MT_ERR_UNSUPPORTED_DTYPE;
+  if (add && res_dtype != act_dtype && res_dtype != MT_F32) return MT_ERR_UNSUPPORTED_DTYPE;
+  if (act_dtype != MT_F32 && act_dtype != MT_F16 && act_dtype != MT_BF16) return MT_ERR_UNSUPPORTED_DTYPE;
+  if (rows == 0) return MT_OK;
+  if (hidden == nullptr || w == nullptr || q == nullptr || scale == nullptr || (add && new_residual == nullptr))
+    return MT_ERR_INVALID_ARGUMENT;
+  if ((st = bind_device_of(hidden)) != MT_OK) return st;
+  QParams p{hidden, residual, w, w_dtype == MT_F32, new_residual, q, scale, rows, (int)dim, eps};
+  auto s = static_cast<cudaStream_t>(stream);
+  const bool wide = add && res_dtype == MT_F32;
+  switch (act_dtype) {
+    case MT_F32: return add ? dispatch<float, float, kAddNorm>(p, s) : dispatch<float, float, kNorm>(p, s);
+    case MT_F16:
+      if (!add) return dispatch<__half, __half, kNorm>(p, s);
+      return wide ? dispatch<__half, float, kAddNorm>(p, s) : dispatch<__half, __half, kAddNorm>(p, s);
+    default:
+      if (!add) return dispatch<__nv_bfloat16, __nv_bfloat16, kNorm>(p, s);
+      return wide ? dispatch<__nv_bfloat16, float, kAddNorm>(p, s)
+                  : dispatch<__nv_bfloat16, __nv_bfloat16, kAddNorm>(p, s);
+  }
+}
+
+extern "C" int mt_quantize_rows_int8(const void* x, int dtype, int8_t* q, float* scale, int64_t rows, int64_t dim,
+                                     void* stream) {
+  int st = check_shape(rows, dim);
+  if (st != MT_OK) return st;
+  if (dtype != MT_F32 && dtype != MT_F16 && dtype != MT_BF16) return MT_ERR_UNSUPPORTED_DTYPE;
+  if (rows == 0) return MT_OK;
+  if (x == nullptr || q == nullptr || scale == nullptr) return MT_ERR_INVALID_ARGUMENT;
+  if ((st = bind_device_of(x)) != MT_OK) return st;
+  QParams p{x, nullptr, nullptr, 0, nullptr, q, scale, rows, (int)dim, 0.f};
+  auto s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case MT_F32: return dispatch<float, float, kPlain>(p, s);
+    case MT_F16: return dispatch<__half, __half, kPlain>(p, s);
+    default: return dispatch<__nv_bfloat16, __nv_bfloat16, kPlain>(p, s);
+  }
+}
