@@ -350,6 +350,29 @@ MT_API int mt_fused_ce_bwd(const void* hidden, const void* weight, const void* l
                            void* stream);
 
 /* ---------------------------------------------------------------------
+ * Token embedding   replaces the nn.Embedding lookup and its gradient
+ *   (src/mega_trading/model.py:58, :93)
+ *   out[i, :] = round(scale * weight[ids[i], :])
+ *   dweight[v, :] = round(scale * sum_{i: ids[i] = v} dout[i, :])
+ * ids: n int64 (ids_i64 = 1) or int32; weight [vocab, dim], out / dout [n, dim],
+ * dweight [vocab, dim], contiguous, each fp32, bf16 or fp16.  The gradient is
+ * dense (rows no id names become zero), summed in fp32 in an order that depends
+ * on the ids alone.  Ids equal to padding_idx (negative: none) add to no
+ * gradient.  Ids outside [0, vocab) give a zero output row, add to no gradient
+ * and set the status word ((7 << 16) | 0xEEEE).
+ * n, vocab < 2^31.  workspace: mt_embedding_bwd_workspace_bytes() bytes,
+ * 256-byte aligned.
+ * ------------------------------------------------------------------- */
+MT_API int mt_embedding_fwd(const void* ids, int ids_i64, int64_t n, const void* weight,
+                            int w_dtype, int64_t vocab, int64_t dim, float scale, void* out,
+                            int out_dtype, uint32_t* status, void* stream);
+MT_API int64_t mt_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t dim);
+MT_API int mt_embedding_bwd(const void* ids, int ids_i64, int64_t n, const void* dout,
+                            int dout_dtype, int64_t vocab, int64_t dim, float scale,
+                            int64_t padding_idx, void* dweight, int dw_dtype, void* workspace,
+                            int64_t workspace_bytes, uint32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------
  * 8-bit rows: RMSNorm (with the residual add) and plain quantisation to int8
  *   with one fp32 scale per row.  Inference only.  No counterpart in the
  *   reference (bf16 projections).

@@ -91,6 +91,14 @@ PROTOTYPES: dict[str, tuple[object, list[object]]] = {
          c_i64p, c_i64p, c_i64p, c_i64p, c_i64p, c_i64p, c_i64p, c_float, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp,
          c_vp],
     ),
+    "mt_embedding_fwd": (
+        c_int, [c_vp, c_int, c_i64, c_vp, c_int, c_i64, c_i64, c_float, c_vp, c_int, c_vp, c_vp],
+    ),
+    "mt_embedding_bwd_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
+    "mt_embedding_bwd": (
+        c_int,
+        [c_vp, c_int, c_i64, c_vp, c_int, c_i64, c_i64, c_float, c_i64, c_vp, c_int, c_vp, c_i64, c_vp, c_vp],
+    ),
     "mt_rms_norm_int8": (
         c_int,
         [c_vp, c_int, c_vp, c_int, c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_float, c_vp],
@@ -181,6 +189,15 @@ def status_word(device: torch.device) -> torch.Tensor:
     return t
 
 
+def status_ptr(device: torch.device, op: str) -> int:
+    """Address of the device's status word; refuses to create it inside a stream capture
+    (it would belong to the graph's memory and be cleared by every replay)."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    if idx not in _status and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{op}: call an sm_100a operator once on this device before capturing a graph")
+    return status_word(device).data_ptr()
+
+
 def read_status(device: torch.device) -> int:
     """Return and clear the device status word (synchronises the device)."""
     t = status_word(device)
@@ -192,12 +209,14 @@ def read_status(device: torch.device) -> int:
 
 # kernel ids of the status word's high half (the kKernelId constants in csrc/)
 KERNEL_NAMES = {1: "attention forward", 2: "attention backward", 3: "fused cross-entropy", 4: "fused cross-entropy",
-                6: "projection GEMM", 9: "8-bit matrix product", 15: "wait probe"}
+                6: "projection GEMM", 7: "token embedding", 9: "8-bit matrix product", 15: "wait probe"}
 
 
 def describe_status(code: int) -> str:
     """Text for a nonzero device status word: which kernel gave up and where."""
     kid, site = code >> 16, code & 0xFFFF
+    if site == 0xEEEE and kid == 7:
+        return f"{KERNEL_NAMES[kid]}: a token id is out of range [0, vocab)"
     if site == 0xEEEE:
         return f"{KERNEL_NAMES.get(kid, f'kernel {kid}')}: a target label is out of range [0, vocab)"
     if site == 0xFFFF:

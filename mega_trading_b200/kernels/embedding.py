@@ -1,0 +1,90 @@
+"""Token embedding with a scale on sm_100a, and its gradient by sorted tokens.
+
+Reference: ``nn.Embedding`` of the model (duoan/mega-trading
+``src/mega_trading/model.py:58, :93``).  The lookup, the scale (models that
+multiply their embeddings by ``sqrt(dim)``) and the rounding to the output
+dtype are one pass.  The gradient sorts the token positions by id and sums the
+neighbouring rows in fp32: it is dense, written completely, rounded once to the
+weight's dtype, and the same bits every time (torch's own gradient adds with
+atomics).
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+
+__all__ = ["scaled_embedding"]
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class _ScaledEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx, out_dtype):
+        lib = _lib.load()
+        w, idc = weight.contiguous(), ids.contiguous()
+        vocab, dim = w.shape
+        dev = w.device
+        out = torch.empty((*ids.shape, dim), device=dev, dtype=out_dtype)
+        with torch.cuda.device(dev):
+            st = lib.mt_embedding_fwd(
+                idc.data_ptr(), 1 if idc.dtype == torch.int64 else 0, idc.numel(), w.data_ptr(),
+                _lib.dtype_code(w.dtype), vocab, dim, scale, out.data_ptr(), _lib.dtype_code(out_dtype),
+                _lib.status_ptr(dev, "scaled_embedding"), _lib.stream_ptr(dev),
+            )
+        _lib.check(st, "scaled_embedding forward")
+        ctx.save_for_backward(idc)
+        ctx.args = (scale, padding_idx, vocab, dim, weight.dtype)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        if not ctx.needs_input_grad[0]:
+            return None, None, None, None, None
+        lib = _lib.load()
+        (ids,) = ctx.saved_tensors
+        scale, padding_idx, vocab, dim, wdtype = ctx.args
+        g = grad_output.contiguous()
+        dev = g.device
+        n = ids.numel()
+        dw = torch.empty((vocab, dim), device=dev, dtype=wdtype)
+        ws = torch.empty((int(lib.mt_embedding_bwd_workspace_bytes(n, vocab, dim)),), device=dev, dtype=torch.uint8)
+        with torch.cuda.device(dev):
+            st = lib.mt_embedding_bwd(
+                ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, n, g.data_ptr(), _lib.dtype_code(g.dtype),
+                vocab, dim, scale, padding_idx, dw.data_ptr(), _lib.dtype_code(wdtype), ws.data_ptr(), ws.numel(),
+                _lib.status_ptr(dev, "scaled_embedding"), _lib.stream_ptr(dev),
+            )
+        _lib.check(st, "scaled_embedding backward")
+        return dw, None, None, None, None
+
+
+def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: int | None = None,
+                     out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``scale * weight[ids]`` in ``out_dtype`` (the weight's by default), differentiable in ``weight``.
+
+    ``ids``: int32 or int64 of any shape; ``weight``: [vocab, dim] fp32, bf16 or fp16; the result has
+    shape ``[*ids.shape, dim]``.  Places holding ``padding_idx`` (which may count from the end) look up
+    their row but add to no gradient.  An id outside ``[0, vocab)`` gives a row of zeros, adds to no
+    gradient and sets the device status word (:func:`mega_trading_b200._lib.check_status`)."""
+    op = "scaled_embedding"
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError("weight must have shape [vocab, dim] with at least one row and column")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError("ids must be an int32 or int64 tensor")
+    out_dtype = out_dtype or weight.dtype
+    if weight.dtype not in _FLOATS or out_dtype not in _FLOATS:
+        raise RuntimeError(f"{op} takes and writes float32, bfloat16 or float16")
+    pad = -1
+    if padding_idx is not None:
+        if not -weight.shape[0] <= padding_idx < weight.shape[0]:
+            raise ValueError("padding_idx must be within the vocabulary")
+        pad = int(padding_idx) % weight.shape[0]
+    _lib.require_cuda_sm100(weight, op)
+    if ids.device != weight.device:
+        raise RuntimeError(f"{op} requires ids and weight on one device, found {ids.device} and {weight.device}")
+    return _ScaledEmbedding.apply(weight, ids, float(scale), pad, out_dtype)

@@ -148,7 +148,7 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     with torch.cuda.device(x.device):
         st = _lib.load().mt_int8_gemm(
             xc.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _lib.dtype_code(out_dtype),
-            x.numel() // k, n, k, _lib.status_word(x.device).data_ptr(), _lib.stream_ptr(x.device),
+            x.numel() // k, n, k, _lib.status_ptr(x.device, op), _lib.stream_ptr(x.device),
         )
     _lib.check(st, op)
     return y

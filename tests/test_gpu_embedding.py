@@ -1,0 +1,213 @@
+"""Token embedding and its gradient against the definition in 64 bits.
+
+Forward: one fp32 product and one rounding (half a step of the output type).
+Gradient: fp32 sums.  A run of up to 64 rows is added in sequence and the
+partial sums of a longer run again in sequence, so with c tokens on a row the
+sum of its terms carries at most (min(c, 64) + c / 32 + 10) roundings of 2^-24
+of the sum of magnitudes; the scale adds one and the output type half a step.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _ids(n, vocab, kind, g):
+    if kind == "same":
+        return torch.full((n,), vocab // 2, dtype=torch.long)
+    if kind == "skewed":
+        return (torch.rand(n, generator=g).pow(4) * vocab).long().clamp_(max=vocab - 1)
+    if kind == "ordered":
+        return torch.arange(n) % vocab
+    return torch.randint(0, vocab, (n,), generator=g)
+
+
+def _check_grad(dw, ids, grad, vocab, scale, pad):
+    """dw against the 64-bit sums, with the bound of the module docstring."""
+    g = grad.double()
+    keep = torch.ones_like(ids, dtype=torch.bool) if pad is None else ids != pad
+    keep &= (ids >= 0) & (ids < vocab)
+    g = g * keep.unsqueeze(1)
+    idx = ids.clamp(0, vocab - 1)
+    zero = torch.zeros(vocab, g.shape[1], device=g.device, dtype=torch.float64)
+    ref = zero.index_add(0, idx, g) * scale
+    mag = zero.index_add(0, idx, g.abs()) * abs(scale)
+    c = torch.bincount(idx[keep], minlength=vocab).double().unsqueeze(1)
+    half = torch.finfo(dw.dtype).eps / 2
+    tol = (c.clamp(max=64) + c / 32 + 11) * 2.0 ** -24 * mag + half * ref.abs() \
+        + torch.finfo(dw.dtype).smallest_normal * torch.finfo(dw.dtype).eps
+    bad = (dw.double() - ref).abs() > tol * 1.0001
+    assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[:4].tolist())
+    assert bool((dw[c[:, 0] == 0] == 0).all())
+
+
+@pytest.mark.parametrize("n,vocab,dim,kind,wt,ot,scale,pad,seed", [
+    (1, 21504, 768, "uniform", F32, F32, 1.0, None, 1),
+    (16, 21504, 768, "uniform", F32, BF16, 27.7, None, 2),
+    (4096, 21504, 256, "skewed", F32, F32, 1.0, None, 3),     # the largest single-block sort
+    (4097, 21504, 256, "skewed", F32, F32, 1.0, None, 4),     # the smallest tiled sort
+    (20000, 21504, 768, "skewed", F32, F32, 1.0, 0, 5),
+    (30011, 1000, 1000, "uniform", BF16, BF16, 31.6, 999, 6),
+    (5000, 300, 509, "uniform", F16, F16, 0.5, None, 7),      # odd width: single-element accesses
+    (5000, 300, 510, "skewed", F32, F16, 2.0, 17, 8),
+    (70000, 70000, 16, "uniform", F32, F32, 1.0, None, 9),    # three radix passes
+    (9000, 1, 40, "same", F32, F32, 1.0, None, 10),           # one row
+    (9000, 2, 8, "uniform", BF16, F32, 1.0, 1, 11),
+    (50000, 21504, 64, "same", F32, F32, 1.0, None, 12),      # one token takes the whole stream
+    (3000, 255, 12, "same", F32, BF16, -1.5, None, 13),
+    (21504, 21504, 32, "ordered", F32, F32, 1.0, None, 14),   # every id once
+    (1100000, 21504, 8, "skewed", F32, F32, 1.0, 3, 15),      # tiles of several sub-tiles
+    (33, 7, 1, "uniform", F16, F32, 1.0, None, 16),
+    (40000, 5, 2050, "uniform", BF16, BF16, 1.0, None, 17),   # long runs, many slabs
+])
+def test_embedding_matches_definition(cuda_device, n, vocab, dim, kind, wt, ot, scale, pad, seed):
+    from mega_trading_b200 import _lib
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    g = torch.Generator().manual_seed(seed)
+    ids = _ids(n, vocab, kind, g).to(cuda_device)
+    w = (torch.randn(vocab, dim, generator=g) * 0.5).to(cuda_device, wt).requires_grad_()
+    grad = torch.randn(n, dim, generator=g).to(cuda_device, ot)
+    y = scaled_embedding(ids, w, scale=scale, padding_idx=pad, out_dtype=ot)
+    assert y.dtype == ot and y.shape == (n, dim)
+    # one product in fp32, one rounding: torch's elementwise operations give the same bits
+    assert torch.equal(y, (w.detach()[ids].float() * scale).to(ot))
+    y.backward(grad)
+    assert w.grad.dtype == wt
+    _check_grad(w.grad, ids, grad, vocab, scale, pad)
+    dw = w.grad.clone()
+    w.grad = None
+    scaled_embedding(ids, w, scale=scale, padding_idx=pad, out_dtype=ot).backward(grad)
+    assert torch.equal(w.grad, dw)  # fixed order of the sums
+    assert _lib.read_status(cuda_device) == 0
+
+
+def test_embedding_gradient_against_differences(cuda_device):
+    """The loss is linear in the table, so a finite difference along a direction is the
+    gradient's inner product with it, up to rounding."""
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    ids = torch.randint(0, 50, (700,), device=cuda_device, generator=g)
+    w = torch.randn(50, 24, device=cuda_device, generator=g).requires_grad_()
+    r = torch.randn(700, 24, device=cuda_device, generator=g)
+    d = torch.randn(50, 24, device=cuda_device, generator=g)
+    scaled_embedding(ids, w, scale=3.0).backward(r)
+    with torch.no_grad():
+        hi = (scaled_embedding(ids, w + d, scale=3.0).double() * r.double()).sum()
+        lo = (scaled_embedding(ids, w - d, scale=3.0).double() * r.double()).sum()
+    want = float((hi - lo) / 2)
+    got = float((w.grad.double() * d.double()).sum())
+    # 700 * 24 terms of magnitude ~3, each with relative rounding below 2^-22
+    assert abs(got - want) <= 700 * 24 * 30 * 2.0 ** -22
+
+
+def test_embedding_shapes_and_layouts(cuda_device):
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    w = torch.randn(40, 64, device=cuda_device, generator=g)
+    ids = torch.randint(0, 40, (3, 5, 7), device=cuda_device, generator=g)
+    want = w[ids]
+    assert torch.equal(scaled_embedding(ids, w), want)
+    assert torch.equal(scaled_embedding(ids.int(), w), want)
+    assert torch.equal(scaled_embedding(ids.transpose(0, 2), w), w[ids.transpose(0, 2)])
+    assert torch.equal(scaled_embedding(ids[0, 0, 0], w), w[ids[0, 0, 0]])  # a single id without dimensions
+    big = torch.randn(40, 131, device=cuda_device, generator=g)
+    view = big[:, 3:67]
+    assert torch.equal(scaled_embedding(ids, view), view[ids])
+    off = torch.randn(40 * 64 + 1, device=cuda_device, generator=g)[1:].view(40, 64)  # off the 16-byte grid
+    assert torch.equal(scaled_embedding(ids, off), off[ids])
+    # gradients that arrive expanded (a sum) or transposed
+    wl = w.clone().requires_grad_()
+    scaled_embedding(ids, wl, padding_idx=-40).sum().backward()
+    counts = torch.bincount(ids.flatten(), minlength=40).float()
+    counts[0] = 0
+    assert torch.equal(wl.grad, counts[:, None].expand(40, 64))
+    wl.grad = None
+    y = scaled_embedding(ids, wl)
+    gr = torch.randn(64, 7, 5, 3, device=cuda_device, generator=g).permute(3, 2, 1, 0)
+    y.backward(gr)
+    _check_grad(wl.grad, ids.flatten(), gr.reshape(-1, 64), 40, 1.0, None)
+
+
+def test_embedding_empty(cuda_device):
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    w = torch.randn(11, 8, device=cuda_device, requires_grad=True)
+    y = scaled_embedding(torch.empty(0, 3, dtype=torch.long, device=cuda_device), w)
+    assert y.shape == (0, 3, 8)
+    y.sum().backward()
+    assert bool((w.grad == 0).all())
+
+
+def test_embedding_out_of_range_ids_set_the_status_word(cuda_device):
+    from mega_trading_b200 import _lib
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    for n in (100, 6000):
+        g = torch.Generator(device=cuda_device).manual_seed(n)
+        ids = torch.randint(0, 30, (n,), device=cuda_device, generator=g)
+        ids[3], ids[50], ids[99] = 30, -1, 2 ** 40
+        w = torch.randn(30, 16, device=cuda_device, generator=g).requires_grad_()
+        assert _lib.read_status(cuda_device) == 0
+        y = scaled_embedding(ids, w)
+        code = _lib.read_status(cuda_device)
+        assert code == (7 << 16) | 0xEEEE and "token id is out of range" in _lib.describe_status(code)
+        assert bool((y[[3, 50, 99]] == 0).all())
+        grad = torch.randn(n, 16, device=cuda_device, generator=g)
+        y.backward(grad)
+        assert _lib.read_status(cuda_device) == (7 << 16) | 0xEEEE
+        _check_grad(w.grad, ids, grad, 30, 1.0, None)
+        with pytest.raises(_lib.B200KernelError, match="token id"):
+            scaled_embedding(ids, w)
+            _lib.check_status(cuda_device)
+
+
+def test_embedding_infinities_stay_in_their_rows(cuda_device):
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    ids = torch.tensor([1, 2, 1, 3, 9], device=cuda_device)
+    w = torch.zeros(10, 8, device=cuda_device, requires_grad=True)
+    grad = torch.ones(5, 8, device=cuda_device)
+    grad[1] = float("inf")
+    grad[4] = float("nan")
+    scaled_embedding(ids, w, padding_idx=9).backward(grad)
+    assert bool((w.grad[1] == 2).all()) and bool(w.grad[2].isinf().all()) and bool((w.grad[3] == 1).all())
+    assert bool((w.grad[9] == 0).all()) and bool((w.grad[0] == 0).all())  # a NaN at a padded place is not read
+
+
+def test_embedding_in_a_graph_and_on_another_stream(cuda_device):
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    ids = torch.randint(0, 500, (6000,), device=cuda_device, generator=g)
+    w = torch.randn(500, 72, device=cuda_device, generator=g).requires_grad_()
+    grad = torch.randn(6000, 72, device=cuda_device, generator=g)
+
+    def step():
+        y = scaled_embedding(ids, w, scale=2.0)
+        return y.detach(), torch.autograd.grad(y, w, grad)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            y1, d1 = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y2, d2 = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y1, y2) and torch.equal(d1, d2)
+    ids.copy_(torch.randint(0, 500, (6000,), device=cuda_device, generator=g))
+    graph.replay()
+    torch.cuda.synchronize()
+    y3, d3 = step()
+    assert torch.equal(y2, y3) and torch.equal(d2, d3) and not torch.equal(d2, d1)

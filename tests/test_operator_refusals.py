@@ -52,3 +52,35 @@ def test_int8_wrappers_refuse_cpu_tensors():
         int8.quantize_rows_int8(x)
     with pytest.raises(RuntimeError, match="CUDA"):
         int8.int8_linear(q, torch.ones(2), q, torch.ones(2))
+
+
+def test_embedding_refusals():
+    from mega_trading_b200 import _lib
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    lib = _lib.load()
+    f32 = _lib.MT_F32
+    fwd, bwd = lib.mt_embedding_fwd, lib.mt_embedding_bwd
+    assert fwd(FAKE, 1, -1, FAKE, f32, 10, 8, 1.0, FAKE, f32, FAKE, None) == 1
+    assert fwd(FAKE, 1, 4, FAKE, f32, 0, 8, 1.0, FAKE, f32, FAKE, None) == 1
+    assert fwd(FAKE, 1, 4, FAKE, 5, 10, 8, 1.0, FAKE, f32, FAKE, None) == 2
+    assert fwd(FAKE, 1, 4, FAKE, f32, 10, 8, 1.0, FAKE, f32, None, None) == 1
+    assert fwd(FAKE, 1, 2 ** 31, FAKE, f32, 10, 8, 1.0, FAKE, f32, FAKE, None) == 1
+    assert fwd(None, 1, 0, None, f32, 10, 8, 1.0, None, f32, None, None) == 0
+    need = lib.mt_embedding_bwd_workspace_bytes(5000, 300, 64)
+    assert need >= 2 * 5000 * 8
+    assert bwd(FAKE, 1, 5000, FAKE, f32, 300, 64, 1.0, -1, FAKE, f32, FAKE, need - 1, FAKE, None) == 7
+    assert bwd(FAKE, 1, 5000, FAKE, f32, 300, 64, 1.0, -1, FAKE, f32, ODD, need, FAKE, None) == 7
+    assert bwd(FAKE, 1, 5000, FAKE, f32, 300, 64, 1.0, 300, FAKE, f32, FAKE, need, FAKE, None) == 1
+    assert bwd(FAKE, 1, 5000, FAKE, f32, 300, 64, 1.0, -1, None, f32, FAKE, need, FAKE, None) == 1
+    ids, w = torch.zeros(3, dtype=torch.long), torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        scaled_embedding(ids, w)
+    with pytest.raises(ValueError, match="ids must be"):
+        scaled_embedding(ids.float(), w)
+    with pytest.raises(ValueError, match="weight must have shape"):
+        scaled_embedding(ids, w[0])
+    with pytest.raises(ValueError, match="padding_idx"):
+        scaled_embedding(ids, w, padding_idx=4)
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        scaled_embedding(ids, w, out_dtype=torch.float64)
