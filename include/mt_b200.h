@@ -350,6 +350,50 @@ MT_API int mt_fused_ce_bwd(const void* hidden, const void* weight, const void* l
                            void* stream);
 
 /* ---------------------------------------------------------------------
+ * Distillation loss of an output projection against a teacher's top logits.
+ *   No counterpart in the reference.
+ *     p = softmax(teacher_logits / temperature) over a row's unmasked entries
+ *     q = softmax(hidden weight^T / temperature) over the vocabulary
+ *     loss = temperature^2 * mean over rows with an entry of
+ *            sum_j p_j (log p_j - log q[teacher_ids_j])
+ * hidden [N, K], weight [V, K] bf16 or fp16 (dtype), contiguous, 16-byte
+ * aligned, K % 8 == 0; teacher_ids [N, top] int64 (ids_i64 = 1) or int32,
+ * teacher_logits [N, top] in logits_dtype, contiguous, 1 <= top <= 256, in any
+ * order, ids may repeat.  An entry whose id is ignore_index is masked: its
+ * logit is not used, whatever it holds.  Ids outside [0, V) are masked too and
+ * set the status word ((8 << 16) | 0xEEEE).  Rows without an entry of finite
+ * weight (all masked, or all logits -inf) add neither loss nor gradient; loss
+ * is 0 without any row.  The logits exist in TMEM only.
+ * Outputs kept for the backward: list_ids / list_probs / list_logits [N, top]
+ * (a row's entries by rising id, equal ids merged, INT32_MAX past the last),
+ * row_stats [N + 3] = per-row log2 of the softmax sum (+inf: no entry),
+ * {loss, rows, 1 / rows}.
+ * ------------------------------------------------------------------- */
+MT_API int64_t mt_distill_workspace_bytes(int64_t N, int64_t V);
+MT_API int mt_distill_fwd(const void* hidden, const void* weight, int dtype,
+                          const void* teacher_ids, int ids_i64, int64_t ignore_index,
+                          const void* teacher_logits, int logits_dtype, int64_t N, int64_t V,
+                          int64_t K, int64_t top, float temperature, float* loss, int* list_ids,
+                          float* list_probs, float* list_logits, float* row_stats,
+                          void* workspace, int64_t workspace_bytes, uint32_t* status,
+                          void* stream);
+
+/* Backward: dz = (q - p) * temperature * grad_out / rows;  dhidden = dz weight,
+ * dweight = dz^T hidden.  dz is rounded to dtype (once, after the subtraction)
+ * and exists for one chunk of rows at a time in the workspace
+ * (mt_distill_bwd_workspace_bytes(), 256-byte aligned: at most 512 MB of dz
+ * plus fp32 partial sums); sums are fp32 in a fixed order.  grad_out: device
+ * fp32 scalar.  dhidden [N, K] / dweight [V, K] contiguous, 16-byte aligned,
+ * in dh_dtype / dw_dtype; either may be NULL to skip it. */
+MT_API int64_t mt_distill_bwd_workspace_bytes(int64_t N, int64_t V, int64_t K);
+MT_API int mt_distill_bwd(const void* hidden, const void* weight, int dtype, int64_t N, int64_t V,
+                          int64_t K, int64_t top, float temperature, const int* list_ids,
+                          const float* list_probs, const float* list_logits,
+                          const float* row_stats, const float* grad_out, void* dhidden,
+                          int dh_dtype, void* dweight, int dw_dtype, void* workspace,
+                          int64_t workspace_bytes, uint32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------
  * Token embedding   replaces the nn.Embedding lookup and its gradient
  *   (src/mega_trading/model.py:58, :93)
  *   out[i, :] = round(scale * weight[ids[i], :])

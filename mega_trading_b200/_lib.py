@@ -91,6 +91,18 @@ PROTOTYPES: dict[str, tuple[object, list[object]]] = {
          c_i64p, c_i64p, c_i64p, c_i64p, c_i64p, c_i64p, c_i64p, c_float, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp,
          c_vp],
     ),
+    "mt_distill_workspace_bytes": (c_i64, [c_i64, c_i64]),
+    "mt_distill_fwd": (
+        c_int,
+        [c_vp, c_vp, c_int, c_vp, c_int, c_i64, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_float, c_vp, c_vp, c_vp,
+         c_vp, c_vp, c_vp, c_i64, c_vp, c_vp],
+    ),
+    "mt_distill_bwd_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
+    "mt_distill_bwd": (
+        c_int,
+        [c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_float, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp,
+         c_int, c_vp, c_i64, c_vp, c_vp],
+    ),
     "mt_embedding_fwd": (
         c_int, [c_vp, c_int, c_i64, c_vp, c_int, c_i64, c_i64, c_float, c_vp, c_int, c_vp, c_vp],
     ),
@@ -209,7 +221,8 @@ def read_status(device: torch.device) -> int:
 
 # kernel ids of the status word's high half (the kKernelId constants in csrc/)
 KERNEL_NAMES = {1: "attention forward", 2: "attention backward", 3: "fused cross-entropy", 4: "fused cross-entropy",
-                6: "projection GEMM", 7: "token embedding", 9: "8-bit matrix product", 15: "wait probe"}
+                6: "projection GEMM", 7: "token embedding", 8: "distillation loss",
+                9: "8-bit matrix product", 15: "wait probe"}
 
 
 def describe_status(code: int) -> str:
@@ -217,6 +230,8 @@ def describe_status(code: int) -> str:
     kid, site = code >> 16, code & 0xFFFF
     if site == 0xEEEE and kid == 7:
         return f"{KERNEL_NAMES[kid]}: a token id is out of range [0, vocab)"
+    if site == 0xEEEE and kid == 8:
+        return f"{KERNEL_NAMES[kid]}: a teacher id is out of range [0, vocab)"
     if site == 0xEEEE:
         return f"{KERNEL_NAMES.get(kid, f'kernel {kid}')}: a target label is out of range [0, vocab)"
     if site == 0xFFFF:

@@ -1,0 +1,717 @@
+// Distillation loss of an output projection against a teacher's top logits.
+//
+//   p_r = softmax(t_r / T) over the row's listed entries that are not masked
+//   q_r = softmax(h_r W^T / T) over the whole vocabulary
+//   loss = T^2 * mean over rows with an entry of  sum_j p_rj (log p_rj - log q_r[id_rj])
+//   dz_r = (q_r - scatter(p_r)) * T / n_rows,   dh = dz W,   dW = dz^T h
+//
+// No counterpart in the reference, which trains against labels only.
+//
+// Forward: the logits' row statistics come from the fused cross-entropy's
+// product (fused_ce.cu: logits only in TMEM).  distill_prep_kernel turns a
+// row's list into its probabilities, sorted by id with equal ids merged, and
+// distill_row_kernel forms the loss.
+//
+// Backward: dz is needed by two products with different reductions (dh over
+// the vocabulary, dW over the rows).  Recomputing the logits once per product
+// on chip costs 8 N V K operations; writing dz out once costs 6 N V K and
+// 2 bytes per logit, so rows are taken in chunks whose 16-bit dz fits in a
+// bounded workspace:
+//   1. dz chunk = round(2^(z log2e / T - lse)) (tile product, epilogue)
+//   2. listed entries are overwritten with round(q - p) from the forward's
+//      fp32 logits: the difference is rounded once, not its parts
+//   3. dh chunk = dz W        (W read along its rows, no transposed copy)
+//   4. dW      += dz^T h      (fp32, both operands read along their rows)
+// q - p is kept without the factor T * grad / n, which the epilogues apply in
+// fp32: it would push 16-bit values of a mean over many rows out of range.
+// fp16 values are held times 2^15 for the same reason (|q - p| <= 1).  The rounding of
+// dz to 16 bits (half a step of its own magnitude) is the tensor cores' operand
+// type and the one rounding between the fp32 logits and the fp32 sums.
+#include <cmath>
+
+#include "fused_ce.cuh"
+#include "tile_gemm.cuh"
+
+namespace mt {
+namespace {
+
+constexpr uint32_t kKernelId = 8;
+constexpr int kMaxTop = 256;
+constexpr int kNone = 0x7fffffff;  // id of an unused list slot
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// ---------------------------------------------------------------------------
+// the teacher's lists
+// ---------------------------------------------------------------------------
+struct PrepParams {
+  const void* ids;
+  int ids_i64;
+  const void* logits;
+  int64_t ignore_index;
+  int N, V, top;
+  float temp;
+  int* tid;      // [N, top] ids in rising order, kNone past the last
+  float* tp;     // [N, top] their probabilities (0 past the last)
+  float* ent;    // [N] sum p log p; NaN-free for empty rows (0)
+  float* mass;   // [N] 1 for a row with an entry, else 0
+  uint32_t* status;
+};
+
+// One warp per row.
+template <typename TL>
+__global__ void __launch_bounds__(256) distill_prep_kernel(const PrepParams p) {
+  __shared__ int s_id[8][kMaxTop];
+  __shared__ int o_id[8][kMaxTop];
+  __shared__ float o_p[8][kMaxTop];
+  const int lane = lane_id(), w = warp_id();
+  const int64_t row = int64_t(blockIdx.x) * 8 + w;
+  if (row >= p.N) return;
+  const int top = p.top;
+  constexpr int kPer = kMaxTop / 32;
+  float a[kPer];
+  int id[kPer];
+  float mx = -INFINITY;
+  bool odd = false;  // an id outside the vocabulary
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int j = i * 32 + lane;
+    id[i] = kNone;
+    a[i] = -INFINITY;
+    if (j < top) {
+      const int64_t at = row * top + j;
+      const int64_t v = p.ids_i64 ? static_cast<const int64_t*>(p.ids)[at]
+                                  : (int64_t) static_cast<const int32_t*>(p.ids)[at];
+      if (v >= 0 && v < p.V && v != p.ignore_index) {
+        id[i] = (int)v;
+        a[i] = __fdiv_rn(to_f32<TL>(static_cast<const TL*>(p.logits)[at]), p.temp);
+        mx = fmaxf(mx, a[i]);
+      } else if (v != p.ignore_index) {
+        odd = true;
+      }
+      s_id[w][j] = id[i];
+    }
+  }
+  if (odd) atomicCAS(p.status, 0u, (kKernelId << 16) | 0xEEEEu);
+  mx = warp_max(mx);
+  // a list of -inf only has no mass: the row counts as empty.  (A NaN logit
+  // keeps mx finite or -inf and makes the sum NaN.)
+  float e[kPer], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    e[i] = id[i] != kNone ? expf(a[i] - mx) : 0.f;
+    sum += e[i];
+  }
+  sum = warp_sum(sum);
+  const bool nan_row = __any_sync(0xffffffffu, [&] {
+    bool b = false;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) b |= id[i] != kNone && isnan(a[i]);
+    return b;
+  }());
+  const bool live = mx > -INFINITY || nan_row;
+  const float lse = logf(sum);
+  float ent = 0.f;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int j = i * 32 + lane;
+    if (i * 32 >= top) break;
+    const float pr = live && id[i] != kNone ? __fdiv_rn(e[i], sum) : 0.f;
+    if (pr != 0.f) ent += pr * (a[i] - mx - lse);
+    if (j < top) {
+      // place in the order of (id, position)
+      int rank = 0;
+      const int mine = id[i];
+      for (int q = 0; q < top; ++q) {
+        const int other = s_id[w][q];
+        rank += other < mine || (other == mine && q < j);
+      }
+      o_id[w][rank] = live ? mine : kNone;
+      o_p[w][rank] = pr;
+    }
+  }
+  ent = warp_sum(ent);
+  __syncwarp();
+  // merge equal ids into the first of them and close the gaps
+  int kept = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (i * 32 >= top) break;
+    const int j = i * 32 + lane;
+    const int mine = j < top ? o_id[w][j] : kNone;
+    const bool head = mine != kNone && (j == 0 || o_id[w][j - 1] != mine);
+    const uint32_t heads = __ballot_sync(0xffffffffu, head);
+    if (head) {
+      float s = o_p[w][j];
+      for (int q = j + 1; q < top && o_id[w][q] == mine; ++q) s += o_p[w][q];
+      const int at = kept + __popc(heads & ((1u << lane) - 1u));
+      p.tid[row * top + at] = mine;
+      p.tp[row * top + at] = s;
+    }
+    kept += __popc(heads);
+  }
+  for (int j = kept + lane; j < top; j += 32) {
+    p.tid[row * top + j] = kNone;
+    p.tp[row * top + j] = 0.f;
+  }
+  if (lane == 0) {
+    p.ent[row] = live ? ent : 0.f;
+    p.mass[row] = live ? 1.f : 0.f;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// per-row loss
+// ---------------------------------------------------------------------------
+struct RowParams {
+  const void* hidden;
+  const void* weight;
+  int N, K, top, splits;
+  const float* part_m;
+  const float* part_s;
+  const int* tid;
+  const float* tp;
+  const float* ent;
+  const float* mass;
+  float inv_temp;
+  float* zt;     // [N, top] logits of the listed entries
+  float* lse2;   // [N] log2 of the row's sum, +inf for rows without an entry
+  float* part;   // [blocks, 2] sums of loss and of rows
+};
+
+// One warp per row: the listed logits (dot products in fp32), the row's loss,
+// and the block's partial sums in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256) distill_row_kernel(const RowParams p) {
+  __shared__ float red[2][8];
+  const int lane = lane_id(), w = warp_id();
+  const int64_t row = int64_t(blockIdx.x) * 8 + w;
+  float loss = 0.f, count = 0.f;
+  if (row < p.N) {
+    float M = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_m[row * p.splits + s]);
+    float S = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float m = p.part_m[row * p.splits + s];
+      if (m != -INFINITY) S += p.part_s[row * p.splits + s] * exp2f(m - M);
+    }
+    const float l2 = M + log2f(S);
+    const bool live = p.mass[row] != 0.f;
+    const T* h = static_cast<const T*>(p.hidden) + row * p.K;
+    float cross = 0.f;
+    if (live) {
+      for (int j = 0; j < p.top; ++j) {
+        const int id = p.tid[row * p.top + j];
+        if (id == kNone) break;
+        const T* v = static_cast<const T*>(p.weight) + int64_t(id) * p.K;
+        float z = 0.f;
+        for (int k = lane * 8; k < p.K; k += 256) {
+          float x[8], y[8];
+          load_vec<T, 8>(h + k, x);
+          load_vec<T, 8>(v + k, y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) z = fmaf(x[e], y[e], z);
+        }
+        z = warp_sum(z);
+        if (lane == 0) p.zt[row * p.top + j] = z;
+        const float pr = p.tp[row * p.top + j];
+        if (pr != 0.f) cross += pr * (z * p.inv_temp - l2 * kLn2);
+      }
+      loss = p.ent[row] - cross;
+      count = 1.f;
+    }
+    if (lane == 0) p.lse2[row] = live ? l2 : INFINITY;
+  }
+  if (lane == 0) {
+    red[0][w] = loss;
+    red[1][w] = count;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += red[threadIdx.x][i];
+    p.part[int64_t(blockIdx.x) * 2 + threadIdx.x] = s;
+  }
+}
+
+// loss = T^2 * sum / rows (0 without rows); scal = {loss, rows, 1 / rows}
+__global__ void __launch_bounds__(1024) distill_loss_kernel(const float* __restrict__ part, int n, float temp,
+                                                            float* __restrict__ scal, float* __restrict__ loss) {
+  __shared__ float sl[32], sv[32];
+  float l = 0.f, v = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const float2 q = __ldg(reinterpret_cast<const float2*>(part) + i);
+    l += q.x;
+    v += q.y;
+  }
+  l = warp_sum(l);
+  v = warp_sum(v);
+  if (lane_id() == 0) {
+    sl[warp_id()] = l;
+    sv[warp_id()] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    l = warp_sum(sl[threadIdx.x]);
+    v = warp_sum(sv[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      const float inv = v > 0.f ? 1.f / v : 0.f;
+      const float r = v > 0.f ? temp * temp * l * inv : 0.f;
+      scal[0] = r;
+      scal[1] = v;
+      scal[2] = inv;
+      loss[0] = r;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+// 16-bit q times `up` (a power of two), columns past the vocabulary zero.
+template <typename T>
+struct SoftmaxEpilogue {
+  static constexpr uint32_t kKernelId = mt::kKernelId;
+  static constexpr int OUT_SIZE = 2;
+  const float* lse2;
+  float zscale;
+  float log2_up;
+  bool add, direct;
+
+  struct Row {
+    float shift;  // log2(up) - lse2, or -inf for a row without an entry
+  };
+  __device__ __forceinline__ Row row(int m, bool live) const {
+    return Row{live ? log2_up - __ldg(lse2 + m) : -INFINITY};
+  }
+  __device__ __forceinline__ void pack(const uint32_t (&z)[32], const Row& r, int, uint32_t* words) const {
+    const bool some = r.shift != -INFINITY;  // NaN logits of a row without an entry stay out
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float a = fast_exp2(fmaf(__uint_as_float(z[i]), zscale, r.shift));
+      const float b = fast_exp2(fmaf(__uint_as_float(z[i + 1]), zscale, r.shift));
+      words[i >> 1] = some ? pack2<T>(a, b) : 0u;
+    }
+  }
+};
+
+// accumulator * temp * grad_out / rows / up
+template <typename TO>
+struct GradEpilogue {
+  static constexpr uint32_t kKernelId = mt::kKernelId;
+  static constexpr int OUT_SIZE = sizeof(TO);
+  const float* inv_rows;
+  const float* grad_out;
+  float factor;  // temp / up
+  bool add, direct;
+
+  struct Row {
+    float g;
+  };
+  __device__ __forceinline__ Row row(int, bool) const { return Row{factor * __ldg(grad_out) * __ldg(inv_rows)}; }
+  __device__ __forceinline__ void pack(const uint32_t (&z)[32], const Row& r, int, uint32_t* words) const {
+    if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) words[i] = __float_as_uint(__uint_as_float(z[i]) * r.g);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i += 2)
+        words[i >> 1] = pack2<TO>(__uint_as_float(z[i]) * r.g, __uint_as_float(z[i + 1]) * r.g);
+    }
+  }
+};
+
+// Listed entries of a chunk of rows: dz = round((q - p) * up).
+template <typename T>
+__global__ void __launch_bounds__(256) distill_listed_kernel(const int* __restrict__ tid, const float* __restrict__ tp,
+                                                             const float* __restrict__ zt,
+                                                             const float* __restrict__ lse2, uint32_t n, uint32_t top,
+                                                             float zscale, float up, T* __restrict__ dz, int64_t ld) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int id = tid[i];
+  if (id == kNone) return;
+  const uint32_t row = i / top;
+  const float q = fast_exp2(fmaf(zt[i], zscale, -lse2[row]));
+  dz[int64_t(row) * ld + id] = from_f32<T>((q - tp[i]) * up);
+}
+
+// out = sum over splits of part (fixed order), cast to out's dtype; 4 columns a thread.
+template <typename TO>
+__global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict__ part, int splits,
+                                                         int64_t split_elems, int64_t n4, TO* __restrict__ out) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n4; i += int64_t(gridDim.x) * 256) {
+    float4 a = __ldg(reinterpret_cast<const float4*>(part) + i);
+    for (int s = 1; s < splits; ++s) {
+      const float4 b = __ldg(reinterpret_cast<const float4*>(part + s * split_elems) + i);
+      a.x += b.x;
+      a.y += b.y;
+      a.z += b.z;
+      a.w += b.w;
+    }
+    if constexpr (sizeof(TO) == 4)
+      reinterpret_cast<float4*>(out)[i] = a;
+    else
+      reinterpret_cast<uint2*>(out)[i] = make_uint2(pack2<TO>(a.x, a.y), pack2<TO>(a.z, a.w));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+
+struct FwdPlan {
+  int splits;
+  int64_t blocks, off_m, off_s, off_ent, off_mass, off_part, bytes;
+};
+FwdPlan plan_fwd(int64_t N, int64_t V) {
+  FwdPlan pl;
+  pl.splits = logit_stats_splits(N, V);
+  pl.blocks = (N + 7) / 8;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += up256(bytes);
+    return o;
+  };
+  pl.off_m = take(N * pl.splits * 4);
+  pl.off_s = take(N * pl.splits * 4);
+  pl.off_ent = take(N * 4);
+  pl.off_mass = take(N * 4);
+  pl.off_part = take(pl.blocks * 8);
+  pl.bytes = at;
+  return pl;
+}
+
+// No split without a stage: every partial sum that is read was written.
+int even_splits(int64_t k_stages, int64_t splits) {
+  const int64_t per = (k_stages + splits - 1) / splits;
+  return (int)((k_stages + per - 1) / per);
+}
+
+// Splits of the inner dimension (k_stages stages of 64): the split that ends
+// soonest counted in stages over whole waves of CTA pairs, where a tile costs
+// about 4 stages of pipeline fill and drain and every split's partial sums are
+// written and read again.
+int choose_k_splits(int64_t tiles, int64_t k_stages) {
+  const int64_t units = std::max<int64_t>(1, get_sm_count() / 2);
+  int best = 1;
+  double best_cost = 1e30;
+  const int64_t most = std::min<int64_t>(64, std::max<int64_t>(1, k_stages / 4));
+  for (int64_t s = 1; s <= most; ++s) {
+    const int64_t per = (k_stages + s - 1) / s;
+    const int64_t waves = (tiles * s + units - 1) / units;
+    const double cost = double(waves) * double(per + 4) + (s > 1 ? 4.0 + 0.15 * double(s) : 0.0);
+    if (cost < best_cost * 0.98) {
+      best_cost = cost;
+      best = (int)s;
+    }
+  }
+  return even_splits(k_stages, best);
+}
+
+constexpr int64_t kDzBytes = int64_t(512) << 20;  // most of the workspace: one chunk's dz
+
+struct BwdPlan {
+  int64_t ld;          // dz row stride (elements)
+  int64_t rows;        // rows per chunk
+  int chunks, h_splits, w_splits;
+  int64_t h_pad, w_pad;  // rows of one split's partials
+  int64_t off_dz, off_h, off_w, bytes;
+};
+BwdPlan plan_bwd(int64_t N, int64_t V, int64_t K) {
+  BwdPlan pl;
+  pl.ld = (V + 7) / 8 * 8;
+  const int64_t units = std::max<int64_t>(1, get_sm_count() / 2);
+  const int64_t nt = (K + 255) / 256;
+  // a chunk's dh tiles fill the GPU once, as far as the workspace bound allows
+  int64_t mt = std::max<int64_t>(1, units / nt);
+  mt = std::max<int64_t>(1, std::min<int64_t>(mt, kDzBytes / (pl.ld * 2 * 256)));
+  pl.rows = std::min<int64_t>(N, mt * 256);
+  pl.chunks = (int)((N + pl.rows - 1) / pl.rows);
+  const int64_t h_tiles = (pl.rows + 255) / 256 * nt, w_tiles = (V + 255) / 256 * nt;
+  pl.h_splits = choose_k_splits(h_tiles, (V + 63) / 64);
+  pl.w_splits = choose_k_splits(w_tiles, (pl.rows + 63) / 64);
+  pl.h_pad = (pl.rows + 255) / 256 * 256;
+  pl.w_pad = (V + 255) / 256 * 256;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += up256(bytes);
+    return o;
+  };
+  pl.off_dz = take(pl.rows * pl.ld * 2);
+  pl.off_h = take(pl.h_splits > 1 ? pl.h_splits * pl.h_pad * K * 4 : 0);
+  // fp32 sums of dW: several splits, or several chunks of a 16-bit gradient
+  pl.off_w = take(pl.w_splits * pl.w_pad * K * 4);
+  pl.bytes = at;
+  return pl;
+}
+
+template <int KIND>
+struct Cfgs {
+  using Z = TileCfg<KIND, false, false, 256, true>;   // dz = H W^T
+  using H = TileCfg<KIND, false, true, 256, true>;    // dh = dz W
+  using W = TileCfg<KIND, true, true, 256, true>;     // dW = dz^T H
+};
+
+int sum_splits(const float* part, int splits, int64_t split_elems, int64_t n, void* out, int dtype, cudaStream_t s) {
+  const int64_t n4 = n / 4;  // K is a multiple of 8
+  const int blocks = (int)std::min<int64_t>((n4 + 255) / 256, int64_t(get_sm_count()) * 8);
+  if (dtype == MT_F32)
+    sum_splits_kernel<float><<<blocks, 256, 0, s>>>(part, splits, split_elems, n4, static_cast<float*>(out));
+  else if (dtype == MT_BF16)
+    sum_splits_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(part, splits, split_elems, n4,
+                                                             static_cast<__nv_bfloat16*>(out));
+  else
+    sum_splits_kernel<__half><<<blocks, 256, 0, s>>>(part, splits, split_elems, n4, static_cast<__half*>(out));
+  return check_launch("distill_bwd_sum");
+}
+
+// A gradient product's launch with `dtype` outputs of rows x K.
+template <class C, typename TO>
+int grad_product(const CUtensorMap& a, const CUtensorMap& b, int64_t rows, int64_t K, int64_t k_elems, int splits,
+                 int64_t split_rows, void* out, int dtype, bool add, const float* inv_rows, const float* grad_out,
+                 float factor, uint32_t* status, const char* name, cudaStream_t s) {
+  TileParams<GradEpilogue<TO>> prm;
+  prm.tm_a = a;
+  prm.tm_b = b;
+  const int64_t map_rows = splits > 1 ? splits * split_rows : rows;
+  const int64_t stages = (k_elems + C::BK - 1) / C::BK;
+  // a last chunk with fewer stages leaves the later splits' sums as they are (add)
+  splits = even_splits(stages, splits);
+  int st = tile_output_map(&prm.tm_out, out, dtype, map_rows, K, K);
+  if (st != MT_OK) return st;
+  prm.M = (int)rows;
+  prm.N = (int)K;
+  prm.n_k = (int)stages;
+  prm.k_per_split = (prm.n_k + splits - 1) / splits;
+  prm.split_rows = split_rows;
+  prm.out = out;
+  prm.ld_out = K;
+  prm.status = status;
+  prm.ep = GradEpilogue<TO>{inv_rows, grad_out, factor, add, false};
+  return launch_tile_gemm<C>(prm, splits, name, s);
+}
+
+template <class C>
+int grad_product_as(int dtype, const CUtensorMap& a, const CUtensorMap& b, int64_t rows, int64_t K, int64_t k_elems,
+                    int splits, int64_t split_rows, void* out, bool add, const float* inv_rows, const float* grad_out,
+                    float factor, uint32_t* status, const char* name, cudaStream_t s) {
+  if (dtype == MT_F32)
+    return grad_product<C, float>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows, grad_out,
+                                  factor, status, name, s);
+  if (dtype == MT_BF16)
+    return grad_product<C, __nv_bfloat16>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows,
+                                          grad_out, factor, status, name, s);
+  return grad_product<C, __half>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows, grad_out,
+                                 factor, status, name, s);
+}
+
+struct BwdArgs {
+  const void *hidden, *weight;
+  int64_t N, V, K;
+  int top;
+  float temp;
+  const int* tid;
+  const float *tp, *zt, *lse2, *inv_rows, *grad_out;
+  void* dh;
+  int dh_dtype;
+  void* dw;
+  int dw_dtype;
+  char* ws;
+  uint32_t* status;
+  cudaStream_t s;
+};
+
+template <typename T, int KIND>
+int run_bwd(const BwdArgs& a, const BwdPlan& pl) {
+  using Z = typename Cfgs<KIND>::Z;
+  using H = typename Cfgs<KIND>::H;
+  using W = typename Cfgs<KIND>::W;
+  const float zscale = kLog2e / a.temp;
+  const float log2_up = KIND == kKindF16 ? 15.f : 0.f, up = KIND == kKindF16 ? 32768.f : 1.f;
+  const float factor = a.temp / up;
+  T* dz = reinterpret_cast<T*>(a.ws + pl.off_dz);
+  float* h_part = reinterpret_cast<float*>(a.ws + pl.off_h);
+  float* w_part = reinterpret_cast<float*>(a.ws + pl.off_w);
+  // dW goes straight to its place when one fp32 tensor or one chunk takes it
+  const bool w_direct = pl.w_splits == 1 && (a.dw_dtype == MT_F32 || pl.chunks == 1);
+  int st;
+  for (int c = 0; c < pl.chunks; ++c) {
+    const int64_t r0 = c * pl.rows, rows = std::min(pl.rows, a.N - r0);
+    const T* h = static_cast<const T*>(a.hidden) + r0 * a.K;
+    // 1. q
+    TileParams<SoftmaxEpilogue<T>> zp;
+    if ((st = tile_operand_map<Z>(&zp.tm_a, h, false, rows, a.K, a.K, 128)) != MT_OK) return st;
+    if ((st = tile_operand_map<Z>(&zp.tm_b, a.weight, false, a.V, a.K, a.K, Z::B_ROWS)) != MT_OK) return st;
+    if ((st = tile_output_map(&zp.tm_out, dz, KIND == kKindBf16 ? MT_BF16 : MT_F16, rows, a.V, pl.ld)) != MT_OK)
+      return st;
+    zp.M = (int)rows;
+    zp.N = (int)a.V;
+    zp.n_k = (int)((a.K + Z::BK - 1) / Z::BK);
+    zp.k_per_split = zp.n_k;
+    zp.split_rows = 0;
+    zp.out = dz;
+    zp.ld_out = pl.ld;
+    zp.status = a.status;
+    zp.ep = SoftmaxEpilogue<T>{a.lse2 + r0, zscale, log2_up, false, false};
+    if ((st = launch_tile_gemm<Z>(zp, 1, "distill_bwd_dz", a.s)) != MT_OK) return st;
+    // 2. q - p where the teacher lists an entry
+    const int64_t n = rows * a.top;
+    distill_listed_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, a.s>>>(
+        a.tid + r0 * a.top, a.tp + r0 * a.top, a.zt + r0 * a.top, a.lse2 + r0, (uint32_t)n, (uint32_t)a.top, zscale, up, dz,
+        pl.ld);
+    if ((st = check_launch("distill_bwd_listed")) != MT_OK) return st;
+    // 3. dh = dz W
+    if (a.dh != nullptr) {
+      char* out = static_cast<char*>(a.dh) + r0 * a.K * (a.dh_dtype == MT_F32 ? 4 : 2);
+      CUtensorMap ma, mb;
+      if ((st = tile_operand_map<H>(&ma, dz, false, rows, a.V, pl.ld, 128)) != MT_OK) return st;
+      if ((st = tile_operand_map<H>(&mb, a.weight, true, a.K, a.V, a.K, 0)) != MT_OK) return st;
+      if (pl.h_splits > 1) {
+        if ((st = grad_product_as<H>(MT_F32, ma, mb, rows, a.K, a.V, pl.h_splits, pl.h_pad, h_part, false, a.inv_rows,
+                                     a.grad_out, factor, a.status, "distill_bwd_dh", a.s)) != MT_OK)
+          return st;
+        if ((st = sum_splits(h_part, pl.h_splits, pl.h_pad * a.K, rows * a.K, out, a.dh_dtype, a.s)) != MT_OK)
+          return st;
+      } else if ((st = grad_product_as<H>(a.dh_dtype, ma, mb, rows, a.K, a.V, 1, 0, out, false, a.inv_rows,
+                                          a.grad_out, factor, a.status, "distill_bwd_dh", a.s)) != MT_OK) {
+        return st;
+      }
+    }
+    // 4. dW += dz^T h
+    if (a.dw != nullptr) {
+      CUtensorMap ma, mb;
+      if ((st = tile_operand_map<W>(&ma, dz, true, a.V, rows, pl.ld, 0)) != MT_OK) return st;
+      if ((st = tile_operand_map<W>(&mb, h, true, a.K, rows, a.K, 0)) != MT_OK) return st;
+      if ((st = grad_product_as<W>(w_direct ? a.dw_dtype : MT_F32, ma, mb, a.V, a.K, rows, pl.w_splits, pl.w_pad,
+                                   w_direct ? a.dw : w_part, c > 0, a.inv_rows, a.grad_out, factor, a.status,
+                                   "distill_bwd_dw", a.s)) != MT_OK)
+        return st;
+    }
+  }
+  if (a.dw != nullptr && !w_direct)
+    return sum_splits(w_part, pl.w_splits, pl.w_pad * a.K, a.V * a.K, a.dw, a.dw_dtype, a.s);
+  return MT_OK;
+}
+
+int check_args(const void* hidden, const void* weight, int dtype, int64_t N, int64_t V, int64_t K, int64_t top,
+               float temp) {
+  if (dtype != MT_BF16 && dtype != MT_F16) return MT_ERR_UNSUPPORTED_DTYPE;
+  if (N < 0 || V <= 0 || K <= 0 || top <= 0) return MT_ERR_INVALID_ARGUMENT;
+  if (top > kMaxTop) {
+    set_last_error_text("distillation: at most 256 listed entries per row");
+    return MT_ERR_INVALID_ARGUMENT;
+  }
+  if (!(temp > 0.f) || !std::isfinite(temp)) return MT_ERR_INVALID_ARGUMENT;
+  if (N > 0x7fffffffLL - 256 || V > 0x7fffffffLL - 256 || K > 0x7fffffffLL / 4 - 256) return MT_ERR_INVALID_ARGUMENT;
+  if (N > 0 && (hidden == nullptr || weight == nullptr)) return MT_ERR_INVALID_ARGUMENT;
+  if (K % 8 != 0) return MT_ERR_UNSUPPORTED_LAYOUT;
+  if ((reinterpret_cast<uintptr_t>(hidden) & 15u) || (reinterpret_cast<uintptr_t>(weight) & 15u))
+    return MT_ERR_UNSUPPORTED_LAYOUT;
+  return MT_OK;
+}
+
+bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+}  // namespace
+}  // namespace mt
+
+using namespace mt;
+
+extern "C" int64_t mt_distill_workspace_bytes(int64_t N, int64_t V) {
+  if (N <= 0 || V <= 0) return 256;
+  return plan_fwd(N, V).bytes;
+}
+
+extern "C" int mt_distill_fwd(const void* hidden, const void* weight, int dtype, const void* teacher_ids, int ids_i64,
+                              int64_t ignore_index, const void* teacher_logits, int logits_dtype, int64_t N,
+                              int64_t V, int64_t K, int64_t top, float temperature, float* loss, int* list_ids,
+                              float* list_probs, float* list_logits, float* row_stats, void* workspace,
+                              int64_t workspace_bytes, uint32_t* status, void* stream) {
+  int st = check_args(hidden, weight, dtype, N, V, K, top, temperature);
+  if (st != MT_OK) return st;
+  if (logits_dtype != MT_F32 && logits_dtype != MT_F16 && logits_dtype != MT_BF16) return MT_ERR_UNSUPPORTED_DTYPE;
+  if (loss == nullptr || row_stats == nullptr) return MT_ERR_INVALID_ARGUMENT;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (N == 0) {
+    cudaError_t e = cudaMemsetAsync(loss, 0, 4, s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(row_stats, 0, 12, s);
+    return e == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+  }
+  if (teacher_ids == nullptr || teacher_logits == nullptr || list_ids == nullptr || list_probs == nullptr ||
+      list_logits == nullptr || status == nullptr)
+    return MT_ERR_INVALID_ARGUMENT;
+  const FwdPlan pl = plan_fwd(N, V);
+  if (workspace == nullptr || !aligned_to(workspace, 256) || workspace_bytes < pl.bytes) return MT_ERR_WORKSPACE;
+  if ((st = bind_device_of(hidden)) != MT_OK) return st;
+  if ((st = check_arch()) != MT_OK) return st;
+  char* ws = static_cast<char*>(workspace);
+  float* pm = reinterpret_cast<float*>(ws + pl.off_m);
+  float* ps = reinterpret_cast<float*>(ws + pl.off_s);
+  float* ent = reinterpret_cast<float*>(ws + pl.off_ent);
+  float* mass = reinterpret_cast<float*>(ws + pl.off_mass);
+  float* part = reinterpret_cast<float*>(ws + pl.off_part);
+  const PrepParams pp{teacher_ids, ids_i64, teacher_logits, ignore_index, (int)N, (int)V, (int)top, temperature,
+                      list_ids, list_probs, ent, mass, status};
+  const unsigned blocks = (unsigned)pl.blocks;
+  if (logits_dtype == MT_F32)
+    distill_prep_kernel<float><<<blocks, 256, 0, s>>>(pp);
+  else if (logits_dtype == MT_BF16)
+    distill_prep_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(pp);
+  else
+    distill_prep_kernel<__half><<<blocks, 256, 0, s>>>(pp);
+  if ((st = check_launch("distill_prep")) != MT_OK) return st;
+  if ((st = logit_stats(hidden, weight, dtype, N, V, K, kLog2e / temperature, pl.splits, pm, ps, status, s)) != MT_OK)
+    return st;
+  const RowParams rp{hidden, weight, (int)N, (int)K, (int)top, pl.splits, pm, ps, list_ids, list_probs, ent, mass,
+                     1.f / temperature, list_logits, row_stats, part};
+  if (dtype == MT_BF16)
+    distill_row_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(rp);
+  else
+    distill_row_kernel<__half><<<blocks, 256, 0, s>>>(rp);
+  if ((st = check_launch("distill_row")) != MT_OK) return st;
+  distill_loss_kernel<<<1, 1024, 0, s>>>(part, (int)pl.blocks, temperature, row_stats + N, loss);
+  return check_launch("distill_loss");
+}
+
+extern "C" int64_t mt_distill_bwd_workspace_bytes(int64_t N, int64_t V, int64_t K) {
+  if (N <= 0 || V <= 0 || K <= 0) return 256;
+  return plan_bwd(N, V, K).bytes;
+}
+
+extern "C" int mt_distill_bwd(const void* hidden, const void* weight, int dtype, int64_t N, int64_t V, int64_t K,
+                              int64_t top, float temperature, const int* list_ids, const float* list_probs,
+                              const float* list_logits, const float* row_stats, const float* grad_out, void* dhidden,
+                              int dh_dtype, void* dweight, int dw_dtype, void* workspace, int64_t workspace_bytes,
+                              uint32_t* status, void* stream) {
+  int st = check_args(hidden, weight, dtype, N, V, K, top, temperature);
+  if (st != MT_OK) return st;
+  for (int d : {dh_dtype, dw_dtype})
+    if (d != MT_F32 && d != MT_F16 && d != MT_BF16) return MT_ERR_UNSUPPORTED_DTYPE;
+  if (!aligned_to(dhidden, 16) || !aligned_to(dweight, 16)) return MT_ERR_UNSUPPORTED_LAYOUT;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (N == 0) {
+    if (dweight != nullptr &&
+        cudaMemsetAsync(dweight, 0, size_t(V) * K * (dw_dtype == MT_F32 ? 4 : 2), s) != cudaSuccess)
+      return MT_ERR_LAUNCH;
+    return MT_OK;
+  }
+  if (list_ids == nullptr || list_probs == nullptr || list_logits == nullptr || row_stats == nullptr ||
+      grad_out == nullptr || status == nullptr)
+    return MT_ERR_INVALID_ARGUMENT;
+  const BwdPlan pl = plan_bwd(N, V, K);
+  if (workspace == nullptr || !aligned_to(workspace, 256) || workspace_bytes < pl.bytes) return MT_ERR_WORKSPACE;
+  if (pl.h_splits * pl.h_pad > 0x7fffffffLL || pl.w_splits * pl.w_pad > 0x7fffffffLL) return MT_ERR_INVALID_ARGUMENT;
+  if ((st = bind_device_of(hidden)) != MT_OK) return st;
+  if ((st = check_arch()) != MT_OK) return st;
+  const BwdArgs a{hidden, weight, N, V, K, (int)top, temperature, list_ids, list_probs, list_logits, row_stats,
+                  row_stats + N + 2, grad_out, dhidden, dh_dtype, dweight, dw_dtype, static_cast<char*>(workspace),
+                  status, s};
+  return dtype == MT_BF16 ? run_bwd<__nv_bfloat16, kKindBf16>(a, pl) : run_bwd<__half, kKindF16>(a, pl);
+}

@@ -1,0 +1,325 @@
+"""Distillation loss and its gradients against the definition in 64 bits.
+
+Bounds (u = half a step of the 16-bit type, relative): a logit is an fp32 sum
+of K products, off by at most (K / 16 + 4) 2^-23 |h| |w| (the tensor core adds
+16 products a step, truncating); a probability q is off by a relative
+e = 2 err(z) / T + 1e-4 (the exponential's 2^-22, and the sum of V terms kept
+as running sums of at most a few hundred additions).  dz = q - p is rounded
+once, u |dz|.  The products add (n / 16 + 4) 2^-23 of the sum of magnitudes and
+the output its own half step.  The loss is off by T^2 (2 err(z) / T + 1e-4).
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+IGN = -100
+
+
+def _definition(h, w, ids, logits, temp):
+    """(loss, dz, rows) in 64 bits; h and w in double."""
+    v = w.shape[0]
+    hit = (ids != IGN) & (ids >= 0) & (ids < v)
+    a = torch.where(hit, logits.double() / temp, -float("inf"))
+    alive = (a > -float("inf")).any(1)
+    a = torch.where(alive[:, None], a, torch.zeros_like(a))
+    p = torch.softmax(a, 1) * hit * alive[:, None]
+    logp = torch.where(p > 0, torch.log_softmax(a, 1), torch.zeros_like(a))
+    idx = torch.where(hit, ids, torch.zeros_like(ids)).long()
+    logq = torch.log_softmax((h @ w.t()) / temp, 1)
+    rows = (p * (logp - logq.gather(1, idx))).sum(1)
+    n = max(int(alive.sum()), 1)
+    loss = temp * temp * torch.where(alive, rows, torch.zeros_like(rows)).sum() / n
+    dense = torch.zeros_like(logq).scatter_add(1, idx, p)
+    dz = torch.where(alive[:, None], logq.exp() - dense, torch.zeros_like(logq))
+    q = torch.where(alive[:, None], logq.exp(), torch.zeros_like(logq))
+    return loss, dz, q, n
+
+
+def _run(dev, h, w, ids, logits, temp, dtype, gscale=1.0, compute_weight=None):
+    from mega_trading_b200 import _lib
+    from mega_trading_b200.kernels.distillation import fused_linear_distillation
+
+    hd, wd = h.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = fused_linear_distillation(hd, wd, ids, logits, temperature=temp, ignore_index=IGN,
+                                     compute_weight=compute_weight)
+    assert loss.dtype == F32 and loss.shape == ()
+    dh, dw = torch.autograd.grad(loss, (hd, wd), torch.tensor(gscale, device=dev))
+    assert dh.dtype == h.dtype and dw.dtype == w.dtype
+    assert _lib.read_status(dev) == 0
+    return loss.detach(), dh, dw
+
+
+def _check(h, w, ids, logits, temp, cdtype, gscale, loss, dh, dw):
+    hc, wc = h.to(cdtype).double(), w.to(cdtype).double()
+    ref, dz, q, n = _definition(hc, wc, ids, logits, temp)
+    k, v = hc.shape[1], wc.shape[0]
+    err_z = (k / 16 + 4) * 2.0 ** -23 * float(hc.norm(dim=1).max() * wc.norm(dim=1).max())
+    e = 2 * err_z / temp + 1e-4
+    assert abs(float(loss) - float(ref)) <= temp * temp * e, (float(loss), float(ref))
+    u = torch.finfo(cdtype).eps / 2
+    g = temp * gscale / n
+    dz_err = u * dz.abs() + e * q + 2.0 ** -40
+
+    def close(got, want, mag, mag_err, terms):
+        uo = torch.finfo(got.dtype).eps / 2
+        tiny = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+        tol = abs(g) * (mag_err + (terms / 16 + 4) * 2.0 ** -23 * mag) * (1 + 2 * uo) + uo * want.abs() + tiny
+        bad = (got.double() - want).abs() > tol * 1.0001
+        assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[:4].tolist(),
+                                     float(((got.double() - want).abs() / tol).max()))
+
+    close(dh, g * (dz @ wc), dz.abs() @ wc.abs(), dz_err @ wc.abs(), v)
+    close(dw, g * (dz.t() @ hc), dz.abs().t() @ hc.abs(), dz_err.t() @ hc.abs(), h.shape[0])
+
+
+def _teacher(n, v, top, seed, dev, masked=0.0, empty=0.0):
+    g = torch.Generator(device=dev).manual_seed(seed + 1000)
+    ids = torch.stack([torch.randperm(v, device=dev, generator=g)[:top] for _ in range(min(n, 64))])
+    ids = ids.repeat((n + ids.shape[0] - 1) // ids.shape[0], 1)[:n]
+    ids = (ids + torch.randint(0, v, (n, 1), device=dev, generator=g)) % v
+    logits = torch.randn(n, ids.shape[1], device=dev, generator=g) * 3
+    if masked or empty:
+        gone = torch.rand(ids.shape, device=dev, generator=g) < masked
+        gone |= torch.rand(n, 1, device=dev, generator=g) < empty
+        ids[gone] = IGN
+        logits[gone] = float("nan")
+    return ids, logits
+
+
+@pytest.mark.parametrize("n,v,k,top,temp,dtype,masked,seed", [
+    (1, 21504, 768, 8, 1.0, BF16, 0.0, 1),        # one token
+    (300, 17, 64, 5, 2.0, BF16, 0.2, 2),          # a small vocabulary
+    (77, 1000, 8, 1, 1.0, F16, 0.0, 3),           # the narrowest projection, one listed entry
+    (130, 129, 104, 128, 0.5, BF16, 0.1, 4),
+    (257, 1001, 256, 256, 1.5, F16, 0.3, 5),      # the longest lists, odd vocabulary
+    (509, 21504, 256, 8, 1.0, BF16, 0.2, 6),
+    (700, 21504, 768, 32, 2.0, BF16, 0.0, 7),
+    (640, 21504, 1024, 64, 4.0, F16, 0.1, 8),
+    (6500, 1500, 768, 16, 1.0, BF16, 0.1, 9),     # two chunks of rows
+    (5000, 2000, 1032, 16, 2.0, F16, 0.1, 10),    # two chunks, five column tiles
+    (20000, 300, 256, 33, 1.0, BF16, 0.1, 11),    # two chunks of a narrow student
+    (64, 120000, 128, 20, 1.0, BF16, 0.0, 12),    # a large vocabulary
+])
+def test_distillation_matches_definition(cuda_device, n, v, k, top, temp, dtype, masked, seed):
+    g = torch.Generator(device=cuda_device).manual_seed(seed)
+    h = torch.randn(n, k, device=cuda_device, generator=g).to(dtype)
+    w = (torch.randn(v, k, device=cuda_device, generator=g) * 0.05).to(dtype)
+    ids, logits = _teacher(n, v, top, seed, cuda_device, masked, masked / 2)
+    gscale = float(n)  # loss scaling: fp16 gradients of a mean stay in range
+    out = _run(cuda_device, h, w, ids, logits, temp, dtype, gscale)
+    _check(h, w, ids, logits, temp, dtype, gscale, *out)
+    again = _run(cuda_device, h, w, ids, logits, temp, dtype, gscale)
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
+
+
+def test_distillation_gradient_of_a_close_student(cuda_device):
+    """A peaked student near its teacher: q and p nearly cancel where the mass is, and the
+    gradient must be as exact as the difference, not as its parts."""
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    n, v, k = 200, 900, 64
+    h = (torch.randn(n, k, device=cuda_device, generator=g)).to(BF16)
+    w = (torch.randn(v, k, device=cuda_device, generator=g) * 0.8).to(BF16)
+    z = h.double() @ w.double().t()
+    logits, ids = z.topk(100, dim=1)
+    logits = (logits + 0.01 * torch.randn(logits.shape, device=cuda_device, generator=g)).float()
+    out = _run(cuda_device, h, w, ids, logits, 1.0, BF16)
+    _check(h, w, ids, logits, 1.0, BF16, 1.0, *out)
+
+
+def test_distillation_gradients_against_differences(cuda_device):
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    n, v, k, temp = 40, 60, 32, 1.7
+    h = torch.randn(n, k, device=cuda_device, generator=g).to(BF16)
+    w = (torch.randn(v, k, device=cuda_device, generator=g) * 0.3).to(BF16)
+    ids, logits = _teacher(n, v, 7, 2, cuda_device, 0.2, 0.1)
+    _, dh, dw = _run(cuda_device, h, w, ids, logits, temp, BF16)
+    for leaf, grad in ((0, dh), (1, dw)):
+        x = [h.double(), w.double()]
+        d = torch.randn(x[leaf].shape, device=cuda_device, generator=g).double()
+        step = 1e-4
+        ends = []
+        for sign in (1, -1):
+            y = list(x)
+            y[leaf] = y[leaf] + sign * step * d
+            ends.append(float(_definition(y[0], y[1], ids, logits, temp)[0]))
+        want = (ends[0] - ends[1]) / (2 * step)
+        got = float((grad.double() * d).sum())
+        # dz and the output each carry at most a relative 2^-8; the magnitudes bound the sum
+        _, dz, _, rows = _definition(x[0], x[1], ids, logits, temp)
+        m = (dz.abs() @ x[1].abs()) if leaf == 0 else (dz.abs().t() @ x[0].abs())
+        assert abs(got - want) <= temp / rows * float((m * d.abs()).sum()) * (2.0 ** -7 + 1e-3) + 1e-6
+
+
+def test_distillation_lists_in_any_order_with_repeats(cuda_device):
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    n, v, k, top = 90, 500, 64, 40
+    h = torch.randn(n, k, device=cuda_device, generator=g).to(BF16)
+    w = (torch.randn(v, k, device=cuda_device, generator=g) * 0.1).to(BF16)
+    ids = torch.randint(0, 25, (n, top), device=cuda_device, generator=g)  # every id about twice
+    ids[0] = 7                                                             # one id only
+    logits = torch.randn(n, top, device=cuda_device, generator=g) * 2
+    out = _run(cuda_device, h, w, ids, logits, 1.0, BF16)
+    _check(h, w, ids, logits, 1.0, BF16, 1.0, *out)
+    # int32 ids and 16-bit logits are the same lists
+    l16 = logits.to(BF16)
+    a = _run(cuda_device, h, w, ids.int(), l16, 1.0, BF16)
+    b = _run(cuda_device, h, w, ids, l16.float(), 1.0, BF16)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    # strided lists
+    wide_i, wide_l = ids.repeat_interleave(2, 1), logits.repeat_interleave(2, 1)
+    c = _run(cuda_device, h, w, wide_i[:, ::2], wide_l[:, ::2], 1.0, BF16)
+    assert all(torch.equal(x, y) for x, y in zip(out, c))
+
+
+def test_distillation_of_one_entry_is_cross_entropy(cuda_device):
+    from mega_trading_b200.kernels.fused_ce import fused_linear_cross_entropy
+
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    h = torch.randn(300, 128, device=cuda_device, generator=g).to(BF16)
+    w = (torch.randn(2000, 128, device=cuda_device, generator=g) * 0.1).to(BF16)
+    labels = torch.randint(0, 2000, (300,), device=cuda_device, generator=g)
+    labels[::9] = IGN
+    loss, dh, dw = _run(cuda_device, h, w, labels[:, None], torch.zeros(300, 1, device=cuda_device), 1.0, BF16)
+    hd, wd = h.clone().requires_grad_(), w.clone().requires_grad_()
+    ce = fused_linear_cross_entropy(hd, wd, labels, ignore_index=IGN)
+    ce.backward()
+    assert abs(float(loss) - float(ce.detach())) <= 1e-4
+    for a, b in ((dh, hd.grad), (dw, wd.grad)):
+        # both round dz once, at different scales: two half steps of it, and two of the output
+        assert float((a.float() - b.float()).norm() / b.float().norm()) <= 4 * 2.0 ** -8
+
+
+def test_distillation_masked_rows_and_lists(cuda_device):
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    n, v, k, top = 140, 300, 64, 6
+    h = torch.randn(n, k, device=cuda_device, generator=g).to(BF16)
+    w = (torch.randn(v, k, device=cuda_device, generator=g) * 0.1).to(BF16)
+    ids, logits = _teacher(n, v, top, 5, cuda_device)
+    logits[0] = -float("inf")                     # no mass at all
+    logits[1, 1:] = -float("inf")                 # all mass on one entry
+    logits[2] = torch.finfo(F32).min              # equal logits, the lowest finite value
+    logits[3, 0] = torch.finfo(F32).max
+    ids[4], logits[4] = IGN, float("inf")         # masked entries may hold anything
+    ids[5, :5] = IGN
+    logits[5, :5] = float("nan")
+    out = _run(cuda_device, h, w, ids, logits, 2.0, BF16)
+    assert all(bool(t.isfinite().all()) for t in out)
+    _check(h, w, ids, logits, 2.0, BF16, 1.0, *out)
+    assert bool((out[1][0] == 0).all()) and bool((out[1][4] == 0).all())
+    # a row without an entry contributes nothing, whatever its logits would be
+    big = h.clone()
+    big[4] = 3e38
+    other = _run(cuda_device, big, w, ids, logits, 2.0, BF16)
+    assert torch.equal(other[0], out[0]) and torch.equal(other[1], out[1])
+    # nothing listed anywhere
+    loss, dh, dw = _run(cuda_device, h, w, torch.full_like(ids, IGN), logits, 2.0, BF16)
+    assert float(loss) == 0.0 and bool((dh == 0).all()) and bool((dw == 0).all())
+
+
+def test_distillation_nan_in_a_listed_logit_reaches_the_loss(cuda_device):
+    h = torch.ones(3, 16, device=cuda_device, dtype=BF16)
+    w = torch.ones(20, 16, device=cuda_device, dtype=BF16)
+    ids = torch.tensor([[1, 2], [3, 4], [5, 6]], device=cuda_device)
+    logits = torch.zeros(3, 2, device=cuda_device)
+    logits[1, 0] = float("nan")
+    loss, dh, _ = _run(cuda_device, h, w, ids, logits, 1.0, BF16)
+    assert bool(loss.isnan()) and bool(dh[1].isnan().any()) and bool(dh[0].isfinite().all())
+
+
+def test_distillation_out_of_range_ids_set_the_status_word(cuda_device):
+    from mega_trading_b200 import _lib
+    from mega_trading_b200.kernels.distillation import fused_linear_distillation
+
+    g = torch.Generator(device=cuda_device).manual_seed(6)
+    h = torch.randn(50, 64, device=cuda_device, generator=g).to(BF16)
+    w = (torch.randn(40, 64, device=cuda_device, generator=g) * 0.1).to(BF16)
+    ids, logits = _teacher(50, 40, 5, 6, cuda_device)
+    clean = ids.clone()
+    ids[3, 2], ids[9, 0], ids[10] = 40, -5, 2 ** 40
+    clean[3, 2] = clean[9, 0] = IGN
+    clean[10] = IGN
+    assert _lib.read_status(cuda_device) == 0
+    hd = h.clone().requires_grad_()
+    loss = fused_linear_distillation(hd, w, ids, logits)
+    loss.backward()
+    code = _lib.read_status(cuda_device)
+    assert code == (8 << 16) | 0xEEEE and "teacher id is out of range" in _lib.describe_status(code)
+    want, dh, _ = _run(cuda_device, h, w, clean, logits, 1.0, BF16)
+    assert torch.equal(loss.detach(), want) and torch.equal(hd.grad, dh)
+
+
+def test_distillation_fp32_master_weight(cuda_device):
+    """fp32 hidden and weight: the kernels read their bf16 roundings, gradients come back in fp32."""
+    g = torch.Generator(device=cuda_device).manual_seed(7)
+    h = torch.randn(150, 72, device=cuda_device, generator=g)
+    w = torch.randn(700, 72, device=cuda_device, generator=g) * 0.1
+    ids, logits = _teacher(150, 700, 9, 7, cuda_device)
+    out = _run(cuda_device, h, w, ids, logits, 1.0, BF16)
+    _check(h, w, ids, logits, 1.0, BF16, 1.0, *out)
+    assert bool((out[2] != out[2].to(BF16).float()).any())
+    copy = _run(cuda_device, h, w, ids, logits, 1.0, BF16, compute_weight=w.to(BF16))
+    assert all(torch.equal(a, b) for a, b in zip(out, copy))
+    # several chunks of rows into an fp32 gradient
+    h2 = torch.randn(9000, 776, device=cuda_device, generator=g)
+    w2 = torch.randn(600, 776, device=cuda_device, generator=g) * 0.05
+    ids, logits = _teacher(9000, 600, 9, 8, cuda_device)
+    out = _run(cuda_device, h2, w2, ids, logits, 1.0, BF16)
+    _check(h2, w2, ids, logits, 1.0, BF16, 1.0, *out)
+
+
+def test_distillation_partial_gradients_and_empty_batch(cuda_device):
+    from mega_trading_b200.kernels.distillation import fused_linear_distillation
+
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    h = torch.randn(70, 64, device=cuda_device, generator=g).to(BF16)
+    w = (torch.randn(90, 64, device=cuda_device, generator=g) * 0.1).to(BF16)
+    ids, logits = _teacher(70, 90, 4, 8, cuda_device)
+    _, dh, dw = _run(cuda_device, h, w, ids, logits, 1.0, BF16)
+    hd = h.clone().requires_grad_()
+    fused_linear_distillation(hd, w, ids, logits.requires_grad_()).backward()
+    assert torch.equal(hd.grad, dh) and logits.grad is None
+    wd = w.clone().requires_grad_()
+    fused_linear_distillation(h, wd, ids, logits.detach()).backward()
+    assert torch.equal(wd.grad, dw)
+    with torch.no_grad():
+        assert not fused_linear_distillation(h, w, ids, logits).requires_grad
+    hd, wd = h[:0].clone().requires_grad_(), w.clone().requires_grad_()
+    loss = fused_linear_distillation(hd, wd, ids[:0], logits[:0].detach())
+    loss.backward()
+    assert float(loss.detach()) == 0.0 and bool((wd.grad == 0).all()) and hd.grad.shape == (0, 64)
+
+
+def test_distillation_in_a_graph_and_on_another_stream(cuda_device):
+    from mega_trading_b200.kernels.distillation import fused_linear_distillation
+
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    h = torch.randn(900, 128, device=cuda_device, generator=g).to(BF16).requires_grad_()
+    w = (torch.randn(1500, 128, device=cuda_device, generator=g) * 0.1).to(BF16).requires_grad_()
+    ids, logits = _teacher(900, 1500, 12, 9, cuda_device)
+
+    def step():
+        loss = fused_linear_distillation(h, w, ids, logits, temperature=2.0)
+        return loss.detach(), *torch.autograd.grad(loss, (h, w))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    with torch.no_grad():
+        h.copy_(torch.randn(900, 128, device=cuda_device, generator=g))
+        logits.copy_(logits.flip(1))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, step()))

@@ -84,3 +84,57 @@ def test_embedding_refusals():
         scaled_embedding(ids, w, padding_idx=4)
     with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
         scaled_embedding(ids, w, out_dtype=torch.float64)
+
+
+def test_distillation_refusals():
+    from mega_trading_b200 import _lib
+    from mega_trading_b200.kernels.distillation import fused_linear_distillation
+
+    lib = _lib.load()
+    f32, bf16 = _lib.MT_F32, _lib.MT_BF16
+    fwd, bwd = lib.mt_distill_fwd, lib.mt_distill_bwd
+
+    def call(hidden=FAKE, dtype=bf16, ldt=f32, n=100, v=500, k=64, top=8, temp=1.0, ws=FAKE, nbytes=1 << 30,
+             status=FAKE):
+        return fwd(hidden, FAKE, dtype, FAKE, 1, -100, FAKE, ldt, n, v, k, top, temp, FAKE, FAKE, FAKE, FAKE, FAKE,
+                   ws, nbytes, status, None)
+
+    assert call(dtype=f32) == 2 and call(ldt=5) == 2
+    assert call(top=0) == 1 and call(top=257) == 1 and call(v=0) == 1 and call(n=-1) == 1
+    assert call(temp=0.0) == 1 and call(temp=-1.0) == 1 and call(temp=float("nan")) == 1
+    assert call(temp=float("inf")) == 1
+    assert call(k=12) == 3 and call(hidden=ODD) == 3
+    assert call(ws=None) == 7 and call(ws=ODD) == 7 and call(nbytes=lib.mt_distill_workspace_bytes(100, 500) - 1) == 7
+    assert call(status=None) == 1
+
+    def back(n=100, top=8, ws=FAKE, nbytes=1 << 40, dhd=bf16, dh=FAKE, go=FAKE):
+        return bwd(FAKE, FAKE, bf16, n, 500, 64, top, 1.0, FAKE, FAKE, FAKE, FAKE, go, dh, dhd, FAKE, bf16, ws, nbytes,
+                   FAKE, None)
+
+    assert back(top=300) == 1 and back(dhd=6) == 2 and back(dh=ODD) == 3 and back(go=None) == 1
+    assert back(ws=None) == 7 and back(nbytes=lib.mt_distill_bwd_workspace_bytes(100, 500, 64) - 1) == 7
+    # the backward's workspace is bounded whatever the batch
+    assert lib.mt_distill_bwd_workspace_bytes(1 << 20, 21504, 768) < 800 << 20
+
+    h, w = torch.randn(4, 8), torch.randn(11, 8)
+    ids, lg = torch.zeros(4, 3, dtype=torch.long), torch.zeros(4, 3)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fused_linear_distillation(h, w, ids, lg)
+    with pytest.raises(ValueError, match="hidden must have shape"):
+        fused_linear_distillation(h[None], w, ids, lg)
+    with pytest.raises(ValueError, match="weight must have shape"):
+        fused_linear_distillation(h, w[:, :4], ids, lg)
+    with pytest.raises(ValueError, match="one row per hidden row"):
+        fused_linear_distillation(h, w, ids[:2], lg[:2])
+    with pytest.raises(ValueError, match="shape of teacher_ids"):
+        fused_linear_distillation(h, w, ids, lg[:, :2])
+    with pytest.raises(ValueError, match="1 to 256"):
+        fused_linear_distillation(h, w, ids[:, :0], lg[:, :0])
+    with pytest.raises(ValueError, match="integer tensor"):
+        fused_linear_distillation(h, w, ids.float(), lg)
+    with pytest.raises(ValueError, match="temperature"):
+        fused_linear_distillation(h, w, ids, lg, temperature=0.0)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        fused_linear_distillation(h[:, :4], w[:, :4], ids, lg)
+    with pytest.raises(ValueError, match="compute_weight"):
+        fused_linear_distillation(h, w, ids, lg, compute_weight=w[:3])
