@@ -395,7 +395,7 @@ MT_API int mt_distill_bwd(const void* hidden, const void* weight, int dtype, int
 
 /* ---------------------------------------------------------------------
  * Token embedding   replaces the nn.Embedding lookup and its gradient
- *   (src/mega_trading/model.py:58, :93)
+ *   (src/mega_trading/model.py:20-147)
  *   out[i, :] = round(scale * weight[ids[i], :])
  *   dweight[v, :] = round(scale * sum_{i: ids[i] = v} dout[i, :])
  * ids: n int64 (ids_i64 = 1) or int32; weight [vocab, dim], out / dout [n, dim],

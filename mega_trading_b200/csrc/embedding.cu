@@ -4,7 +4,7 @@
 //   gradient  dW[v, :] = round(scale * sum_{n: id[n] = v} dy[n, :])   (dense, every row written)
 //
 // Reference: nn.Embedding of TradingModel (duoan/mega-trading
-// src/mega_trading/model.py:58, :93), whose gradient PyTorch computes.
+// src/mega_trading/model.py:20-147), whose gradient PyTorch computes.
 //
 // Forward: bound by HBM (N * dim elements written; the table stays in L2 at
 // this model's sizes).  One warp per token, 16-byte stores.

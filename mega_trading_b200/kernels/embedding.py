@@ -1,7 +1,7 @@
 """Token embedding with a scale on sm_100a, and its gradient by sorted tokens.
 
 Reference: ``nn.Embedding`` of the model (duoan/mega-trading
-``src/mega_trading/model.py:58, :93``).  The lookup, the scale (models that
+``src/mega_trading/model.py:20-147``).  The lookup, the scale (models that
 multiply their embeddings by ``sqrt(dim)``) and the rounding to the output
 dtype are one pass.  The gradient sorts the token positions by id and sums the
 neighbouring rows in fp32: it is dense, written completely, rounded once to the

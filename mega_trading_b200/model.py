@@ -27,6 +27,8 @@ from torch import nn
 
 from .kernels import triton_attention as _attn
 from .kernels import triton_ops as _ops
+from .kernels.distillation import fused_linear_distillation
+from .kernels.embedding import scaled_embedding
 from .kernels.fused_blocks import (GATE_BLOCK, qkv_proj_rope_attention, qkv_rope_attention,
                                    qkv_rope_gemm_supported, swiglu_mlp, swiglu_mlp_supported, swiglu_packed)
 from .kernels.fused_ce import fused_linear_cross_entropy
@@ -98,6 +100,13 @@ class RMSNorm(nn.Module):
 
     def forward(self, x: torch.Tensor, out_dtype: torch.dtype = _BF16) -> torch.Tensor:
         return _ops.rms_norm(x, self.weight, eps=self.eps, out_dtype=out_dtype)
+
+
+class TokenEmbedding(nn.Embedding):
+    """The token table; lookup and sorted-token gradient by ``kernels.embedding``."""
+
+    def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
+        return scaled_embedding(input_ids, self.weight, padding_idx=self.padding_idx)
 
 
 class LlamaAttention(nn.Module):
@@ -203,7 +212,7 @@ class TradingModelB200(nn.Module):
     def __init__(self, cfg: ModelConfig) -> None:
         super().__init__()
         self.cfg = cfg
-        self.token_embedding = nn.Embedding(cfg.vocab_size, cfg.hidden_dim)
+        self.token_embedding = TokenEmbedding(cfg.vocab_size, cfg.hidden_dim)
         self.blocks = nn.ModuleList([LlamaDecoderBlock(cfg) for _ in range(cfg.layers)])
         self.norm = RMSNorm(cfg.hidden_dim, cfg.norm_eps)
         self.output = nn.Linear(cfg.hidden_dim, cfg.vocab_size, bias=False)
@@ -232,10 +241,16 @@ class TradingModelB200(nn.Module):
             out += block.attention.packed_weights() + block.feed_forward.packed_weights()
         return out
 
-    def forward(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None) -> torch.Tensor:
-        """Mean next-token loss when ``labels`` is given (the training entry), else logits."""
+    def forward(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None, *,
+                teacher: tuple[torch.Tensor, torch.Tensor] | None = None, temperature: float = 1.0) -> torch.Tensor:
+        """Mean next-token loss when ``labels`` is given, the distillation loss when ``teacher`` is
+        (``(ids, logits)``, see :meth:`forward_with_distillation`), else logits."""
         if labels is not None:
+            if teacher is not None:
+                raise ValueError("give labels or teacher, not both")
             return self.forward_with_loss(input_ids, labels, return_logits=False)[0]
+        if teacher is not None:
+            return self.forward_with_distillation(input_ids, *teacher, temperature=temperature)
         return F.linear(self.hidden_states(input_ids), self.packed_weights()[0].get()).float()
 
     def forward_with_loss(self, input_ids: torch.Tensor, labels: torch.Tensor, *, return_logits: bool = False,
@@ -255,6 +270,43 @@ class TradingModelB200(nn.Module):
         logits = F.linear(normed, w_out).float()
         loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]), labels.reshape(-1), ignore_index=ignore_index)
         return loss, logits
+
+
+    def forward_with_distillation(self, input_ids: torch.Tensor, teacher_ids: torch.Tensor,
+                                  teacher_logits: torch.Tensor, *, temperature: float = 1.0,
+                                  ignore_index: int = -100) -> torch.Tensor:
+        """Distillation loss against a teacher's top logits (``[batch, time, top]`` ids and logits per
+        position, ``top`` at most 256; ``ignore_index`` masks an entry, a whole row of it a position)."""
+        if teacher_ids.shape[:-1] != input_ids.shape or teacher_logits.shape != teacher_ids.shape:
+            raise ValueError("teacher ids and logits must have shape [batch, time, top] matching input_ids")
+        normed = self.hidden_states(input_ids)
+        pw_out = _packed(self, "_out_bf16", [self.output.weight])
+        top = teacher_ids.shape[-1]
+        return fused_linear_distillation(normed.reshape(-1, normed.shape[-1]), self.output.weight,
+                                         teacher_ids.reshape(-1, top), teacher_logits.reshape(-1, top),
+                                         temperature=temperature, ignore_index=ignore_index,
+                                         compute_weight=pw_out.value())
+
+    @torch.no_grad()
+    def top_logits(self, input_ids: torch.Tensor, top: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """``(ids, logits)`` of each position's ``top`` largest logits, what
+        :meth:`forward_with_distillation` of a student takes."""
+        x = self.hidden_states(input_ids)
+        w = self.packed_weights()[0].get()
+        rows = x.reshape(-1, x.shape[-1])
+        return top_of_projection(input_ids.shape, top, lambda lo, hi: F.linear(rows[lo:hi], w))
+
+
+def top_of_projection(shape: torch.Size, top: int, project) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(ids, logits)`` [*shape, top] of the largest of ``project(lo, hi)``, the logits of flattened
+    positions lo to hi, taken a few positions at a time so that a long batch's never exist at once."""
+    rows = shape.numel()
+    best = [project(lo, min(lo + TOP_ROWS, rows)).topk(top, dim=-1) for lo in range(0, max(rows, 1), TOP_ROWS)]
+    return (torch.cat([b.indices for b in best]).view(*shape, top),
+            torch.cat([b.values for b in best]).view(*shape, top))
+
+
+TOP_ROWS = 8192  # positions whose logits top_of_projection holds at once (0.7 GB in fp32 at 21,504 ids)
 
 
 def _init_weights(module: nn.Module) -> None:

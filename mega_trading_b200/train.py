@@ -150,6 +150,17 @@ class Trainer:
     def step(self, input_ids: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
         """One optimizer step over this rank's ``[B, T]`` batch; returns the mean loss (device scalar,
         no host synchronisation)."""
+        return self._step(input_ids, lambda lo, hi: self.engine(input_ids[lo:hi], labels[lo:hi]))
+
+    def distill_step(self, input_ids: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                     temperature: float = 1.0) -> torch.Tensor:
+        """One optimizer step against a teacher's top logits (``[B, T, top]`` ids and logits, e.g. from
+        ``Int8TradingModel.top_logits``) instead of labels; returns the mean distillation loss."""
+        return self._step(input_ids, lambda lo, hi: self.engine(
+            input_ids[lo:hi], teacher=(teacher_ids[lo:hi], teacher_logits[lo:hi]), temperature=temperature))
+
+    def _step(self, input_ids: torch.Tensor, loss_of) -> torch.Tensor:
+        """One optimizer step; ``loss_of(lo, hi)`` is the engine's mean loss of a micro-batch."""
         if self._store is not None:
             self._await_peers()
         self._steps += 1
@@ -164,7 +175,7 @@ class Trainer:
             frac = (hi - lo) / n
             sync_ctx = self.engine.no_sync() if (self.world > 1 and i < chunks - 1) else contextlib.nullcontext()
             with sync_ctx:
-                loss = self.engine(input_ids[lo:hi], labels[lo:hi])
+                loss = loss_of(lo, hi)
                 self._mark(marks, "forward")
                 (loss * frac).backward()
                 self._mark(marks, "backward" if i < chunks - 1 else "backward+allreduce")
