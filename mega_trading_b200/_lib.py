@@ -180,7 +180,28 @@ def dtype_code(t: torch.dtype) -> int:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    idx = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
+
+
+class _Here:
+    """Context of a call whose device is already current."""
+
+    def __enter__(self) -> None:
+        pass
+
+    def __exit__(self, *exc) -> None:
+        pass
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Context that makes ``device`` current for a launch (nothing to do when it already is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def i64_array(values) -> ctypes.Array:
@@ -205,9 +226,12 @@ def status_ptr(device: torch.device, op: str) -> int:
     """Address of the device's status word; refuses to create it inside a stream capture
     (it would belong to the graph's memory and be cleared by every replay)."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    if idx not in _status and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{op}: call an sm_100a operator once on this device before capturing a graph")
-    return status_word(device).data_ptr()
+    t = _status.get(idx)
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{op}: call an sm_100a operator once on this device before capturing a graph")
+        t = status_word(device)
+    return t.data_ptr()
 
 
 def read_status(device: torch.device) -> int:
@@ -290,12 +314,28 @@ class StatusMonitor:
             self._inspect(h)
 
 
+_sm100: set[int] = set()  # indices of the devices found to be sm_100
+
+
 def require_cuda_sm100(t: torch.Tensor, op: str) -> None:
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{op} requires CUDA tensors (the B200 path has no CPU fallback)")
-    major, minor = torch.cuda.get_device_capability(t.device)
+    idx = t.get_device()
+    if idx in _sm100:
+        return
+    major, minor = torch.cuda.get_device_capability(idx)
     if major != 10 or minor != 0:
         raise RuntimeError(f"{op} requires an sm_100 (B200) GPU, found sm_{major}{minor}")
+    _sm100.add(idx)
+
+
+def require_one_device(op: str, first: torch.Tensor, *others: torch.Tensor) -> None:
+    """All tensors on one sm_100 device."""
+    require_cuda_sm100(first, op)
+    idx = first.get_device()
+    for t in others:
+        if t.get_device() != idx:
+            raise RuntimeError(f"{op} requires all tensors on one device, found {first.device} and {t.device}")
 
 
 def launch_count() -> int:

@@ -41,7 +41,7 @@ class _FusedLinearDistillation(torch.autograd.Function):
         probs, z = torch.empty((2, n, top), device=dev, dtype=torch.float32).unbind(0)
         stats = torch.empty((n + 3,), device=dev, dtype=torch.float32)
         ws = torch.empty((int(lib.mt_distill_workspace_bytes(n, v)),), device=dev, dtype=torch.uint8)
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             st = lib.mt_distill_fwd(
                 h.data_ptr(), w.data_ptr(), _lib.dtype_code(cdtype), ids.data_ptr(),
                 1 if ids.dtype == torch.int64 else 0, ignore_index, logits.data_ptr(), _lib.dtype_code(logits.dtype),
@@ -70,7 +70,7 @@ class _FusedLinearDistillation(torch.autograd.Function):
         dw = torch.empty((v, k), device=dev, dtype=ctx.dtypes[1]) if need_w else None
         go = grad_output.detach().to(device=dev, dtype=torch.float32).reshape(1).contiguous()
         ws = torch.empty((int(lib.mt_distill_bwd_workspace_bytes(n, v, k)),), device=dev, dtype=torch.uint8)
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             st = lib.mt_distill_bwd(
                 h.data_ptr(), w.data_ptr(), _lib.dtype_code(h.dtype), n, v, k, top, ctx.temperature,
                 list_ids.data_ptr(), probs.data_ptr(), z.data_ptr(), stats.data_ptr(), go.data_ptr(),
@@ -125,9 +125,8 @@ def fused_linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teache
         raise ValueError("hidden_dim must be a multiple of 8")
     if compute_weight is not None and compute_weight.shape != weight.shape:
         raise ValueError("compute_weight must have the weight's shape")
-    _lib.require_cuda_sm100(hidden, op)
-    for t in (weight, teacher_ids, teacher_logits, compute_weight):
-        if t is not None and t.device != hidden.device:
-            raise RuntimeError(f"{op} requires all tensors on one device, found {hidden.device} and {t.device}")
+    _lib.require_one_device(op, hidden, weight, teacher_ids, teacher_logits)
+    if compute_weight is not None:
+        _lib.require_one_device(op, hidden, compute_weight)
     return _FusedLinearDistillation.apply(hidden, weight, teacher_ids, teacher_logits, temperature,
                                           int(ignore_index), compute_weight)

@@ -21,23 +21,29 @@ __all__ = ["scaled_embedding"]
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
+def _lookup(weight, ids, scale, out_dtype):
+    """Contiguous ids and the scaled rows."""
+    w, ids = weight.contiguous(), ids.contiguous()
+    vocab, dim = w.shape
+    dev = w.device
+    out = w.new_empty((*ids.shape, dim), dtype=out_dtype)
+    with _lib.on_device(dev):
+        st = _lib.load().mt_embedding_fwd(
+            ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, ids.numel(), w.data_ptr(), _lib.dtype_code(w.dtype),
+            vocab, dim, scale, out.data_ptr(), _lib.dtype_code(out_dtype), _lib.status_ptr(dev, "scaled_embedding"),
+            _lib.stream_ptr(dev),
+        )
+    if st:
+        _lib.check(st, "scaled_embedding forward")
+    return ids, out
+
+
 class _ScaledEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, ids, scale, padding_idx, out_dtype):
-        lib = _lib.load()
-        w, idc = weight.contiguous(), ids.contiguous()
-        vocab, dim = w.shape
-        dev = w.device
-        out = torch.empty((*ids.shape, dim), device=dev, dtype=out_dtype)
-        with torch.cuda.device(dev):
-            st = lib.mt_embedding_fwd(
-                idc.data_ptr(), 1 if idc.dtype == torch.int64 else 0, idc.numel(), w.data_ptr(),
-                _lib.dtype_code(w.dtype), vocab, dim, scale, out.data_ptr(), _lib.dtype_code(out_dtype),
-                _lib.status_ptr(dev, "scaled_embedding"), _lib.stream_ptr(dev),
-            )
-        _lib.check(st, "scaled_embedding forward")
-        ctx.save_for_backward(idc)
-        ctx.args = (scale, padding_idx, vocab, dim, weight.dtype)
+        ids, out = _lookup(weight, ids, scale, out_dtype)
+        ctx.save_for_backward(ids)
+        ctx.args = (scale, padding_idx, *weight.shape, weight.dtype)
         return out
 
     @staticmethod
@@ -51,9 +57,9 @@ class _ScaledEmbedding(torch.autograd.Function):
         g = grad_output.contiguous()
         dev = g.device
         n = ids.numel()
-        dw = torch.empty((vocab, dim), device=dev, dtype=wdtype)
-        ws = torch.empty((int(lib.mt_embedding_bwd_workspace_bytes(n, vocab, dim)),), device=dev, dtype=torch.uint8)
-        with torch.cuda.device(dev):
+        dw = g.new_empty((vocab, dim), dtype=wdtype)
+        ws = g.new_empty((lib.mt_embedding_bwd_workspace_bytes(n, vocab, dim),), dtype=torch.uint8)
+        with _lib.on_device(dev):
             st = lib.mt_embedding_bwd(
                 ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, n, g.data_ptr(), _lib.dtype_code(g.dtype),
                 vocab, dim, scale, padding_idx, dw.data_ptr(), _lib.dtype_code(wdtype), ws.data_ptr(), ws.numel(),
@@ -84,7 +90,7 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 
         if not -weight.shape[0] <= padding_idx < weight.shape[0]:
             raise ValueError("padding_idx must be within the vocabulary")
         pad = int(padding_idx) % weight.shape[0]
-    _lib.require_cuda_sm100(weight, op)
-    if ids.device != weight.device:
-        raise RuntimeError(f"{op} requires ids and weight on one device, found {ids.device} and {weight.device}")
+    _lib.require_one_device(op, weight, ids)
+    if not (weight.requires_grad and torch.is_grad_enabled()):
+        return _lookup(weight, ids, float(scale), out_dtype)[1]
     return _ScaledEmbedding.apply(weight, ids, float(scale), pad, out_dtype)

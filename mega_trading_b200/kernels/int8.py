@@ -29,15 +29,11 @@ MAX_DIM = 32768      # widest row of the quantising operators
 MAX_K = 131056       # longest exact int32 dot product of 8-bit values (a multiple of 16)
 
 
-def _check(op: str, *tensors: torch.Tensor) -> None:
+def _check(op: str, first: torch.Tensor, *others: torch.Tensor) -> None:
     """One CUDA device for all tensors, and no gradient asked of a forward-only operator."""
-    first = tensors[0]
-    _lib.require_cuda_sm100(first, op)
-    for t in tensors:
-        if t.device != first.device:
-            raise RuntimeError(f"{op} requires all tensors on one device, found {first.device} and {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{op} has no gradient; call it under torch.no_grad()")
+    _lib.require_one_device(op, first, *others)
+    if torch.is_grad_enabled() and (first.requires_grad or any(t.requires_grad for t in others)):
+        raise RuntimeError(f"{op} has no gradient; call it under torch.no_grad()")
 
 
 def _rows(op: str, x: torch.Tensor) -> tuple[int, int]:
@@ -52,32 +48,36 @@ def _rows(op: str, x: torch.Tensor) -> tuple[int, int]:
 
 
 def _norm(op: str, hidden, residual, weight, eps: float):
-    tensors = (hidden, weight) if residual is None else (hidden, residual, weight)
-    _check(op, *tensors)
+    if residual is None:
+        _check(op, hidden, weight)
+    else:
+        _check(op, hidden, weight, residual)
     rows, dim = _rows(op, hidden)
-    if weight.dim() != 1 or weight.numel() != dim:
+    act, wdt = hidden.dtype, weight.dtype
+    if weight.dim() != 1 or weight.shape[0] != dim:
         raise ValueError("weight must have one entry per hidden feature")
-    if weight.dtype not in (torch.float32, hidden.dtype):
+    if wdt is not torch.float32 and wdt is not act:
         raise RuntimeError(f"{op} takes a float32 weight or one in the hidden dtype")
     x, w = hidden.contiguous(), weight.contiguous()
-    r = new = None
+    code = rcode = _lib.dtype_code(act)
+    new, r_ptr, new_ptr = None, None, None
     if residual is not None:
         if residual.shape != hidden.shape:
             raise ValueError("hidden and residual must have the same shape")
-        if residual.dtype not in (torch.float32, hidden.dtype):
+        if residual.dtype is not torch.float32 and residual.dtype is not act:
             raise RuntimeError(f"{op} takes a float32 residual or one in the hidden dtype")
         r = residual.contiguous()
         new = torch.empty_like(r)
-    q = torch.empty(hidden.shape, device=x.device, dtype=torch.int8)
-    scale = torch.empty(hidden.shape[:-1], device=x.device, dtype=torch.float32)
-    with torch.cuda.device(x.device):
-        st = _lib.load().mt_rms_norm_int8(
-            x.data_ptr(), _lib.dtype_code(x.dtype), None if r is None else r.data_ptr(),
-            _lib.dtype_code(x.dtype if r is None else r.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
-            None if new is None else new.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, dim, float(eps),
-            _lib.stream_ptr(x.device),
-        )
-    _lib.check(st, op)
+        rcode, r_ptr, new_ptr = _lib.dtype_code(r.dtype), r.data_ptr(), new.data_ptr()
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    dev = x.device
+    with _lib.on_device(dev):
+        st = _lib.load().mt_rms_norm_int8(x.data_ptr(), code, r_ptr, rcode, w.data_ptr(), _lib.dtype_code(wdt),
+                                          new_ptr, q.data_ptr(), scale.data_ptr(), rows, dim, eps,
+                                          _lib.stream_ptr(dev))
+    if st:
+        _lib.check(st, op)
     return new, q, scale
 
 
@@ -109,12 +109,14 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     _check(op, x)
     rows, dim = _rows(op, x)
     xc = x.contiguous()
-    q = torch.empty(x.shape, device=x.device, dtype=torch.int8)
-    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    with torch.cuda.device(x.device):
+    q = xc.new_empty(xc.shape, dtype=torch.int8)
+    scale = xc.new_empty(xc.shape[:-1], dtype=torch.float32)
+    dev = x.device
+    with _lib.on_device(dev):
         st = _lib.load().mt_quantize_rows_int8(xc.data_ptr(), _lib.dtype_code(x.dtype), q.data_ptr(),
-                                               scale.data_ptr(), rows, dim, _lib.stream_ptr(x.device))
-    _lib.check(st, op)
+                                               scale.data_ptr(), rows, dim, _lib.stream_ptr(dev))
+    if st:
+        _lib.check(st, op)
     return q, scale
 
 
@@ -127,11 +129,11 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     a multiple of 16 and at most 131,056."""
     op = "int8_linear"
     _check(op, x, x_scale, weight, weight_scale)
-    if x.dtype != torch.int8 or weight.dtype != torch.int8:
+    if x.dtype is not torch.int8 or weight.dtype is not torch.int8:
         raise RuntimeError("int8_linear takes int8 x and weight")
     if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
         raise ValueError("weight must have shape [out, in] matching x's last dimension")
-    if x_scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
+    if x_scale.dtype is not torch.float32 or weight_scale.dtype is not torch.float32:
         raise RuntimeError("int8_linear takes float32 scales")
     if x_scale.shape != x.shape[:-1]:
         raise ValueError("x_scale must have one entry per row of x")
@@ -143,14 +145,16 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     if k == 0 or k % 16 != 0 or k > MAX_K or n == 0:
         raise ValueError(f"int8_linear needs at least one output and an inner dimension that is a multiple of 16 "
                          f"and at most {MAX_K}")
-    y = torch.empty((*x.shape[:-1], n), device=x.device, dtype=out_dtype)
-    xc, xs, w, ws = (_aligned(t) for t in (x, x_scale, weight, weight_scale))
-    with torch.cuda.device(x.device):
-        st = _lib.load().mt_int8_gemm(
-            xc.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _lib.dtype_code(out_dtype),
-            x.numel() // k, n, k, _lib.status_ptr(x.device, op), _lib.stream_ptr(x.device),
-        )
-    _lib.check(st, op)
+    y = x.new_empty((*x.shape[:-1], n), dtype=out_dtype)
+    xc, w, ws = _aligned(x), _aligned(weight), _aligned(weight_scale)
+    xs = x_scale.contiguous()
+    dev = x.device
+    with _lib.on_device(dev):
+        st = _lib.load().mt_int8_gemm(xc.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(),
+                                      _lib.dtype_code(out_dtype), x.numel() // k, n, k, _lib.status_ptr(dev, op),
+                                      _lib.stream_ptr(dev))
+    if st:
+        _lib.check(st, op)
     return y
 
 
