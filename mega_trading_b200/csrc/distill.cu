@@ -287,7 +287,8 @@ struct SoftmaxEpilogue {
   __device__ __forceinline__ Row row(int m, bool live) const {
     return Row{live ? log2_up - __ldg(lse2 + m) : -INFINITY};
   }
-  __device__ __forceinline__ void pack(const uint32_t (&z)[32], const Row& r, int, uint32_t* words) const {
+  static constexpr bool kCols = false;
+  __device__ __forceinline__ void pack(const uint32_t (&z)[32], const Row& r, const float*, uint32_t* words) const {
     const bool some = r.shift != -INFINITY;  // NaN logits of a row without an entry stay out
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
@@ -312,7 +313,8 @@ struct GradEpilogue {
     float g;
   };
   __device__ __forceinline__ Row row(int, bool) const { return Row{factor * __ldg(grad_out) * __ldg(inv_rows)}; }
-  __device__ __forceinline__ void pack(const uint32_t (&z)[32], const Row& r, int, uint32_t* words) const {
+  static constexpr bool kCols = false;
+  __device__ __forceinline__ void pack(const uint32_t (&z)[32], const Row& r, const float*, uint32_t* words) const {
     if constexpr (sizeof(TO) == 4) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) words[i] = __float_as_uint(__uint_as_float(z[i]) * r.g);
@@ -454,9 +456,9 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t K) {
 
 template <int KIND>
 struct Cfgs {
-  using Z = TileCfg<KIND, false, false, 256, true>;   // dz = H W^T
-  using H = TileCfg<KIND, false, true, 256, true>;    // dh = dz W
-  using W = TileCfg<KIND, true, true, 256, true>;     // dW = dz^T H
+  using Z = TileCfg<KIND, false, false, 256, true, 8>;   // dz = H W^T
+  using H = TileCfg<KIND, false, true, 256, true, 8>;    // dh = dz W
+  using W = TileCfg<KIND, true, true, 256, true, 8>;     // dW = dz^T H
 };
 
 int sum_splits(const float* part, int splits, int64_t split_elems, int64_t n, void* out, int dtype, cudaStream_t s) {

@@ -32,26 +32,27 @@ struct Int8Epilogue {
   };
   __device__ __forceinline__ Row row(int m, bool live) const { return Row{live ? __ldg(xs + m) : 0.f}; }
 
-  __device__ __forceinline__ void pack(const uint32_t (&z)[32], const Row& r, int n0, uint32_t* words) const {
+  static constexpr bool kCols = true;
+  __device__ __forceinline__ float col(int i) const { return i < n ? __ldg(ws + i) : 0.f; }
+
+  __device__ __forceinline__ void pack(const uint32_t (&z)[32], const Row& r, const float* cols,
+                                       uint32_t* words) const {
+    const float2 xs2 = make_float2(r.xs, r.xs);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-      float s[4];
-      if (n0 + j + 4 <= n) {
-        const float4 q = __ldg(reinterpret_cast<const float4*>(ws + n0 + j));  // n0 is a multiple of 32
-        s[0] = q.x; s[1] = q.y; s[2] = q.z; s[3] = q.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = n0 + j + e < n ? __ldg(ws + n0 + j + e) : 0.f;
-      }
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __int2float_rn((int)z[j + e]) * r.xs * s[e];
+      const float4 s = *reinterpret_cast<const float4*>(cols + j);
+      const float2 a = mul2(mul2(make_float2(__int2float_rn((int)z[j]), __int2float_rn((int)z[j + 1])), xs2),
+                            make_float2(s.x, s.y));
+      const float2 b = mul2(mul2(make_float2(__int2float_rn((int)z[j + 2]), __int2float_rn((int)z[j + 3])), xs2),
+                            make_float2(s.z, s.w));
       if constexpr (sizeof(TO) == 4) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) words[j + e] = __float_as_uint(v[e]);
+        words[j] = __float_as_uint(a.x);
+        words[j + 1] = __float_as_uint(a.y);
+        words[j + 2] = __float_as_uint(b.x);
+        words[j + 3] = __float_as_uint(b.y);
       } else {
-        words[j / 2] = pack2<TO>(v[0], v[1]);
-        words[j / 2 + 1] = pack2<TO>(v[2], v[3]);
+        words[j / 2] = pack2<TO>(a.x, a.y);
+        words[j / 2 + 1] = pack2<TO>(b.x, b.y);
       }
     }
   }
@@ -142,8 +143,8 @@ int run_int8(const int8_t* x, const float* xs, const int8_t* w, const float* ws,
   // products take 128 x 128 tiles, four times as many.
   const int64_t pair_tiles = int64_t((M + 255) / 256) * ((N + 255) / 256);
   if (pair_tiles >= get_sm_count() / 2)
-    return launch_tiles<TileCfg<kKindI8, false, false, 256, true>, TO>(x, xs, w, ws, y, out_dtype, M, N, K, status, s);
-  return launch_tiles<TileCfg<kKindI8, false, false, 128, false>, TO>(x, xs, w, ws, y, out_dtype, M, N, K, status, s);
+    return launch_tiles<TileCfg<kKindI8, false, false, 256, true, 16>, TO>(x, xs, w, ws, y, out_dtype, M, N, K, status, s);
+  return launch_tiles<TileCfg<kKindI8, false, false, 128, false, 16>, TO>(x, xs, w, ws, y, out_dtype, M, N, K, status, s);
 }
 
 }  // namespace

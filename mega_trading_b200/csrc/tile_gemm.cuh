@@ -3,9 +3,13 @@
 // B's rows (M and N) are the strided dimension (K-major) or the contiguous
 // one (MN-major, 16-bit types only).
 //
-// Layout of one CTA (320 threads): warps 0-7 epilogue (two warpgroups taking
-// alternate column steps of a tile; thread = row = TMEM lane), warp 8 TMA
-// producer + TMEM allocation, warp 9 MMA issuer.  Tiles are 128 x BN with one
+// Layout of one CTA: EW epilogue warps in warpgroups that take the column steps
+// of a tile in turn (thread = row = TMEM lane), then a TMA producer warp (which
+// also allocates TMEM) and an MMA issuer warp.  EW = 16 puts four epilogue
+// warps on a scheduler to cover each other's TMEM, fence and staging latencies,
+// for products whose epilogue outlasts a tile's main loop with 8 (8-bit, K of
+// about 1,000: 65,537 x 5,632 x 1,024 in 0.42 ms with 8, 0.37 ms with 16); 8
+// leave room for one more stage and poll less.  Tiles are 128 x BN with one
 // CTA, or 256 x BN with a CTA pair (tcgen05 cta_group::2): each CTA of a pair
 // stages its own 128 rows of A and half of B's rows, which takes a third off
 // the shared-memory traffic per product.  A stage of the TMA ring holds 128
@@ -52,13 +56,53 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// Bounded waits whose try_wait may suspend the thread for up to 10 ms before it
+// looks again: the epilogue warps wait through a tile's whole main loop, and
+// polling costs issue slots and power (the distillation step of 32,768 rows runs
+// at the power limit and went from 4.24 to 4.14 ms).
+__device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity, bool cluster) {
+  uint32_t ok;
+  if (cluster)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 0x989680;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 0x989680;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+  return ok != 0;
+}
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait_bounded_long(const WaitCtx& ctx, uint64_t* bar, uint32_t parity, uint32_t site) {
+  if (try_wait_long(bar, parity, CLUSTER)) return true;
+  long long t0 = clock64();
+  while (true) {
+    if (*ctx.abort_flag) return false;
+    if (try_wait_long(bar, parity, CLUSTER)) return true;
+    if (clock64() - t0 > ctx.limit) {
+      atomicCAS(ctx.status, 0u, (ctx.kernel_id << 16) | site);
+      *ctx.abort_flag = 1;
+      return false;
+    }
+  }
+}
+
 // Instruction descriptor, kind::i8: signed 8-bit A and B (K-major), int32 accumulator.
 __host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
-template <int KIND_, bool A_MN_, bool B_MN_, int BN_, bool PAIR_>
+// EW: epilogue warps, 8 or 16.
+template <int KIND_, bool A_MN_, bool B_MN_, int BN_, bool PAIR_, int EW_>
 struct TileCfg {
+  static constexpr int EW = EW_;
+  static constexpr int kThreads = (EW + 2) * 32;
   static constexpr int KIND = KIND_, BN = BN_;
   static constexpr bool A_MN = A_MN_, B_MN = B_MN_, PAIR = PAIR_;
   static_assert(KIND != kKindI8 || (!A_MN && !B_MN), "8-bit operands are K-major");
@@ -70,17 +114,17 @@ struct TileCfg {
   static constexpr int B_BYTES = B_ROWS * 128;
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int BOX = 4096;  // a warp's staging box: 32 rows x 128 bytes
-  static constexpr int OUT_BYTES = 8 * BOX;
-  static constexpr int kMaxStages = (226 * 1024 - OUT_BYTES) / STAGE;
+  static constexpr int OUT_BYTES = EW * BOX;
+  static constexpr int COL_BYTES = EW * 256;  // a warp's 64 per-column values
+  static constexpr int kMaxStages = (226 * 1024 - OUT_BYTES - COL_BYTES) / STAGE;
   static constexpr int NST = kMaxStages < 8 ? kMaxStages : 8;
   static constexpr int OFF_OUT = NST * STAGE;
-  static constexpr int OFF_BAR = OFF_OUT + OUT_BYTES;
+  static constexpr int OFF_COL = OFF_OUT + OUT_BYTES;
+  static constexpr int OFF_BAR = OFF_COL + COL_BYTES;
   static constexpr int SMEM = OFF_BAR + 256;
   static_assert(SMEM <= 227 * 1024, "more shared memory than one sm_100 CTA may use");
   static_assert(2 * NST + 5 <= 28, "mbarriers overlap the TMEM slot");
 };
-
-constexpr int kTileThreads = 320;
 
 template <class EP>
 struct TileParams {
@@ -111,11 +155,14 @@ __device__ __forceinline__ void tma_out(const CUtensorMap* map, const void* src,
 //   static constexpr int OUT_SIZE;          2 or 4 bytes per output element
 //   struct Row;                             per-row values of a tile
 //   Row row(int m, bool live)               loads them
-//   void pack(const uint32_t (&z)[32], const Row&, int n0, uint32_t* words)
-//       32 accumulator columns n0.. -> 16 (OUT_SIZE 2) or 32 (4) packed words
+//   static constexpr bool kCols;            whether per-column values are used
+//   float col(int n)                        loads one (0 past the last column)
+//   void pack(const uint32_t (&z)[32], const Row&, const float* cols, uint32_t* words)
+//       32 accumulator columns and their column values (shared memory) -> 16
+//       (OUT_SIZE 2) or 32 (4) packed words
 //   bool add, direct                        TMA add instead of store; plain stores
 template <class C, class EP>
-__global__ void __launch_bounds__(kTileThreads, 1) tile_gemm_kernel(const __grid_constant__ TileParams<EP> p) {
+__global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_constant__ TileParams<EP> p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   constexpr bool PAIR = C::PAIR;
   constexpr uint32_t kId = EP::kKernelId;
@@ -148,13 +195,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_gemm_kernel(const __grid
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], PAIR ? 16 : 8);  // one arrival per epilogue warp (of both CTAs)
+      mbar_init(&acc_empty[s], (PAIR ? 2 : 1) * C::EW);  // one arrival per epilogue warp (of both CTAs)
     }
     mbar_init(fin, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == C::EW) {
     if constexpr (PAIR) {
       tmem_alloc_pair(tmem_slot, 2 * C::BN);
       tmem_relinquish_pair();
@@ -172,10 +219,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_gemm_kernel(const __grid
   const uint32_t tmem = *tmem_slot;
   const WaitCtx wc{p.status, abort_flag, kId};
   auto wait_x = [&](uint64_t* bar, uint32_t parity, uint32_t site) {
-    if constexpr (PAIR)
-      return wait_bounded_cluster(wc, bar, parity, site);
-    else
-      return wait_bounded(wc, bar, parity, site);
+    return wait_bounded_long<PAIR>(wc, bar, parity, site);
   };
   struct Tile {
     int m0, n0, k0, k1, split;
@@ -187,7 +231,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_gemm_kernel(const __grid
     return Tile{mt * C::TM + row_off, nt * C::BN, k0, min(k0 + p.k_per_split, p.n_k), split};
   };
 
-  if (warp == 8) {
+  if (warp == C::EW) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       tma_prefetch_desc(&p.tm_a);
@@ -239,7 +283,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_gemm_kernel(const __grid
           wait_drain(wc, &full[j % C::NST], (j / C::NST) & 1, 11);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == C::EW + 1) {
     // ------------------------------------------------------------ MMA issuer (even CTA of a pair)
     if (lane == 0 && leader) {
       constexpr uint32_t idesc = C::KIND == kKindI8
@@ -304,10 +348,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_gemm_kernel(const __grid
     // ------------------------------------------------------------ epilogue
     constexpr int kCols = 128 / EP::OUT_SIZE;  // columns of a step
     constexpr int kSub = kCols / 32;
-    const int wg = warp >> 2;         // takes the column steps c with c % 2 == wg
+    constexpr int kSteps = C::BN / kCols;
+    constexpr int kGroups = C::EW / 4;
+    const int wg = warp >> 2;         // takes the column steps c with c % kGroups == wg
     const int r = threadIdx.x & 127;  // row within the tile = TMEM lane
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
     uint8_t* box = smem + C::OFF_OUT + warp * C::BOX;
+    float* cols = reinterpret_cast<float*>(smem + C::OFF_COL) + warp * 64;
     const uint32_t acc_empty_x[2] = {PAIR ? cluster_addr(&acc_empty[0], 0) : 0u,
                                      PAIR ? cluster_addr(&acc_empty[1], 0) : 0u};
     int lt = 0;
@@ -316,33 +363,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_gemm_kernel(const __grid
       const int buf = lt & 1;
       const int m = w.m0 + r;
       const auto rv = p.ep.row(m, m < p.M);
+      auto fetch_cols = [&](int c) {
+        // this step's per-column values, one or two per lane
+        if constexpr (EP::kCols) {
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < kSub; ++h) cols[h * 32 + lane] = p.ep.col(w.n0 + c * kCols + h * 32 + lane);
+          __syncwarp();
+        }
+      };
+      if (wg < kSteps) fetch_cols(wg);
       if (!__all_sync(0xffffffffu, wait_x(&acc_full[buf], (lt >> 1) & 1, 8))) break;
       tc_fence_after();
       const uint32_t acc = tmem + lane_off + buf * C::BN;
       const int warp_row = w.m0 + (warp & 3) * 32;
-#pragma unroll 1
-      for (int c = wg; c < C::BN / kCols; c += 2) {
-        uint32_t words[32];
-#pragma unroll
-        for (int h = 0; h < kSub; ++h) {
-          uint32_t z[32];
-          tmem_ld32(acc + c * kCols + h * 32, z);
-          tmem_ld_wait();
-          if (h == kSub - 1 && c + 2 >= C::BN / kCols) {
-            // last read of this accumulator by this warp
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (PAIR)
-                mbar_arrive_remote(acc_empty_x[buf]);
-              else
-                mbar_arrive(&acc_empty[buf]);
-            }
-          }
-          p.ep.pack(z, rv, w.n0 + c * kCols + h * 32, words + h * 16);
+      auto release = [&]() {
+        // this warp's last read of the accumulator
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR)
+            mbar_arrive_remote(acc_empty_x[buf]);
+          else
+            mbar_arrive(&acc_empty[buf]);
         }
+      };
+      if (wg >= kSteps) release();
+#pragma unroll 1
+      for (int c = wg; c < kSteps; c += kGroups) {
+        uint32_t z[kSub][32];
+#pragma unroll
+        for (int h = 0; h < kSub; ++h) tmem_ld32(acc + c * kCols + h * 32, z[h]);
+        tmem_ld_wait();
+        if (c + kGroups >= kSteps) release();
         const int n0 = w.n0 + c * kCols;
         if (n0 >= p.N) continue;  // nothing of this step exists (warp-uniform)
+        if (c != wg) fetch_cols(c);
+        uint32_t words[32];
+#pragma unroll
+        for (int h = 0; h < kSub; ++h) p.ep.pack(z[h], rv, cols + h * 32, words + h * 16);
         if (lane == 0) bulk_wait_group_read0();  // the box's previous store has left it
         __syncwarp();
 #pragma unroll
@@ -381,7 +440,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_gemm_kernel(const __grid
     cluster_sync_all();
   else
     __syncthreads();
-  if (warp == 8) {
+  if (warp == C::EW) {
     tc_fence_after();
     if constexpr (PAIR)
       tmem_dealloc_pair(tmem, 2 * C::BN);
@@ -437,7 +496,7 @@ int launch_tile_gemm(TileParams<EP>& prm, int splits, const char* name, cudaStre
   if constexpr (C::PAIR) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * 2));
-    cfg.blockDim = dim3(kTileThreads);
+    cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -453,7 +512,7 @@ int launch_tile_gemm(TileParams<EP>& prm, int splits, const char* name, cudaStre
       return MT_ERR_LAUNCH;
     }
   } else {
-    kern<<<units, kTileThreads, C::SMEM, stream>>>(prm);
+    kern<<<units, C::kThreads, C::SMEM, stream>>>(prm);
   }
   return check_launch(name);
 }
