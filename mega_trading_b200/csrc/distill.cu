@@ -7,10 +7,12 @@
 //
 // No counterpart in the reference, which trains against labels only.
 //
-// Forward: the logits' row statistics come from the fused cross-entropy's
-// product (fused_ce.cu: logits only in TMEM).  distill_prep_kernel turns a
-// row's list into its probabilities, sorted by id with equal ids merged, and
-// distill_row_kernel forms the loss.
+// Forward: distill_prep_kernel turns a row's list into its probabilities, sorted
+// by id with equal ids merged.  The tile product keeps a running maximum and sum
+// per row over the vocabulary tiles a CTA pair takes (consecutive ones, so a row
+// is cut over few pairs) and, walking the sorted list along, picks the listed
+// logits out of TMEM: the logits never reach memory.  distill_row_kernel joins
+// the pieces and forms the loss.
 //
 // Backward: dz is needed by two products with different reductions (dh over
 // the vocabulary, dW over the rows).  Recomputing the logits once per product
@@ -29,7 +31,6 @@
 // type and the one rounding between the fp32 logits and the fp32 sums.
 #include <cmath>
 
-#include "fused_ce.cuh"
 #include "tile_gemm.cuh"
 
 namespace mt {
@@ -162,63 +163,118 @@ __global__ void __launch_bounds__(256) distill_prep_kernel(const PrepParams p) {
 }
 
 // ---------------------------------------------------------------------------
+// row statistics of the logits, and the listed logits
+// ---------------------------------------------------------------------------
+struct StatsEpilogue {
+  static constexpr uint32_t kKernelId = mt::kKernelId;
+  static constexpr int OUT_SIZE = 4;
+  static constexpr bool kStats = true;
+  const int* tid;
+  float* zt;
+  float* part_m;  // [N, pieces]: pieces = slots * groups
+  float* part_s;
+  int V, top, pieces, groups, n_nt, per_unit;
+  float zscale;
+
+  struct State {
+    float m, s;          // running maximum (times zscale) and sum of 2^(z zscale - m)
+    int64_t at, end;     // place in the row's list
+    int want, later;     // ids at `at` and after it
+    int64_t piece;       // where the row's statistics go, -1: no such row
+  };
+  __device__ __forceinline__ int id_at(int64_t i, int64_t end) const { return i < end ? __ldg(tid + i) : kNone; }
+
+  __device__ __forceinline__ void begin(State& st, int m, bool live, int mt, int unit, int group) const {
+    st.m = -INFINITY;
+    st.s = 0.f;
+    st.at = int64_t(m) * top;
+    st.end = live ? st.at + top : st.at;
+    st.want = id_at(st.at, st.end);
+    st.later = id_at(st.at + 1, st.end);
+    const int slot = unit - int(int64_t(mt) * n_nt / per_unit);
+    st.piece = live ? int64_t(m) * pieces + slot * groups + group : -1;
+  }
+  __device__ __forceinline__ int next(const State& st) const { return st.want; }
+  __device__ __forceinline__ void skip(State& st) const {
+    ++st.at;
+    st.want = st.later;
+    st.later = id_at(st.at + 1, st.end);
+  }
+  __device__ __forceinline__ void take(State& st, uint32_t z) const {
+    zt[st.at] = __uint_as_float(z);
+    skip(st);
+  }
+  __device__ __forceinline__ void add(State& st, const uint32_t (&z)[32], int n0) const {
+    if (n0 >= V) return;
+    float x[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = n0 + i < V ? __uint_as_float(z[i]) : -INFINITY;
+    float cm = fmaxf(x[0], x[1]);
+#pragma unroll
+    for (int i = 2; i < 32; i += 2) cm = fmax3(cm, x[i], x[i + 1]);
+    const float mn = fmaxf(st.m, cm * zscale);  // zscale > 0
+    const float2 zs = make_float2(zscale, zscale), sh = make_float2(-mn, -mn);
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float2 e = fma2(make_float2(x[i], x[i + 1]), zs, sh);
+      sum = add2(sum, make_float2(fast_exp2(e.x), fast_exp2(e.y)));
+    }
+    st.s = (st.m == -INFINITY ? 0.f : st.s * fast_exp2(st.m - mn)) + (sum.x + sum.y);
+    st.m = mn;
+  }
+  __device__ __forceinline__ void end(const State& st) const {
+    if (st.piece >= 0) {
+      part_m[st.piece] = st.m;
+      part_s[st.piece] = st.s;
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
 // per-row loss
 // ---------------------------------------------------------------------------
 struct RowParams {
-  const void* hidden;
-  const void* weight;
-  int N, K, top, splits;
+  int N, top, pieces, groups, n_nt, per_unit;
   const float* part_m;
   const float* part_s;
   const int* tid;
   const float* tp;
+  const float* zt;
   const float* ent;
   const float* mass;
   float inv_temp;
-  float* zt;     // [N, top] logits of the listed entries
   float* lse2;   // [N] log2 of the row's sum, +inf for rows without an entry
   float* part;   // [blocks, 2] sums of loss and of rows
 };
 
-// One warp per row: the listed logits (dot products in fp32), the row's loss,
-// and the block's partial sums in a fixed order.
-template <typename T>
+// One warp per row; the block's partial sums in a fixed order.
 __global__ void __launch_bounds__(256) distill_row_kernel(const RowParams p) {
   __shared__ float red[2][8];
   const int lane = lane_id(), w = warp_id();
   const int64_t row = int64_t(blockIdx.x) * 8 + w;
   float loss = 0.f, count = 0.f;
   if (row < p.N) {
+    // pieces that exist: the CTA pairs whose tiles cover this row's 256-row tile
+    const int64_t t0 = row / 256 * p.n_nt;
+    const int used = int((t0 + p.n_nt - 1) / p.per_unit - t0 / p.per_unit + 1) * p.groups;
+    const float* pm = p.part_m + row * p.pieces;
+    const float* ps = p.part_s + row * p.pieces;
     float M = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_m[row * p.splits + s]);
+    for (int i = lane; i < used; i += 32) M = fmaxf(M, pm[i]);
+    M = warp_max(M);
     float S = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float m = p.part_m[row * p.splits + s];
-      if (m != -INFINITY) S += p.part_s[row * p.splits + s] * exp2f(m - M);
-    }
-    const float l2 = M + log2f(S);
+    for (int i = lane; i < used; i += 32) S += pm[i] == -INFINITY ? 0.f : ps[i] * exp2f(pm[i] - M);
+    const float l2 = M + log2f(warp_sum(S));
     const bool live = p.mass[row] != 0.f;
-    const T* h = static_cast<const T*>(p.hidden) + row * p.K;
-    float cross = 0.f;
     if (live) {
-      for (int j = 0; j < p.top; ++j) {
-        const int id = p.tid[row * p.top + j];
-        if (id == kNone) break;
-        const T* v = static_cast<const T*>(p.weight) + int64_t(id) * p.K;
-        float z = 0.f;
-        for (int k = lane * 8; k < p.K; k += 256) {
-          float x[8], y[8];
-          load_vec<T, 8>(h + k, x);
-          load_vec<T, 8>(v + k, y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) z = fmaf(x[e], y[e], z);
-        }
-        z = warp_sum(z);
-        if (lane == 0) p.zt[row * p.top + j] = z;
-        const float pr = p.tp[row * p.top + j];
-        if (pr != 0.f) cross += pr * (z * p.inv_temp - l2 * kLn2);
+      float cross = 0.f;
+      for (int j = lane; j < p.top; j += 32) {
+        const int64_t at = row * p.top + j;
+        const float pr = p.tp[at];
+        if (p.tid[at] != kNone && pr != 0.f) cross += pr * (p.zt[at] * p.inv_temp - l2 * kLn2);
       }
-      loss = p.ent[row] - cross;
+      loss = p.ent[row] - warp_sum(cross);
       count = 1.f;
     }
     if (lane == 0) p.lse2[row] = live ? l2 : INFINITY;
@@ -276,6 +332,7 @@ template <typename T>
 struct SoftmaxEpilogue {
   static constexpr uint32_t kKernelId = mt::kKernelId;
   static constexpr int OUT_SIZE = 2;
+  static constexpr bool kStats = false;
   const float* lse2;
   float zscale;
   float log2_up;
@@ -304,6 +361,7 @@ template <typename TO>
 struct GradEpilogue {
   static constexpr uint32_t kKernelId = mt::kKernelId;
   static constexpr int OUT_SIZE = sizeof(TO);
+  static constexpr bool kStats = false;
   const float* inv_rows;
   const float* grad_out;
   float factor;  // temp / up
@@ -366,13 +424,26 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict
 // ---------------------------------------------------------------------------
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
+template <int KIND>
+struct Cfgs {
+  using Z = TileCfg<KIND, false, false, 256, true, 8>;   // H W^T: statistics, dz
+  using H = TileCfg<KIND, false, true, 256, true, 8>;    // dh = dz W
+  using W = TileCfg<KIND, true, true, 256, true, 8>;     // dW = dz^T H
+};
+constexpr int kGroups = 2;  // warpgroups of 8 epilogue warps
+
 struct FwdPlan {
-  int splits;
+  int n_nt, per_unit, pieces;
   int64_t blocks, off_m, off_s, off_ent, off_mass, off_part, bytes;
 };
 FwdPlan plan_fwd(int64_t N, int64_t V) {
   FwdPlan pl;
-  pl.splits = logit_stats_splits(N, V);
+  const int64_t units = std::max<int64_t>(1, get_sm_count() / 2);
+  pl.n_nt = (int)((V + 255) / 256);
+  const int64_t tiles = (N + 255) / 256 * pl.n_nt;
+  pl.per_unit = (int)((tiles + units - 1) / units);
+  // consecutive tiles of one row tile meet at most this many pairs
+  pl.pieces = ((pl.n_nt - 1) / pl.per_unit + 2) * kGroups;
   pl.blocks = (N + 7) / 8;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -380,8 +451,8 @@ FwdPlan plan_fwd(int64_t N, int64_t V) {
     at += up256(bytes);
     return o;
   };
-  pl.off_m = take(N * pl.splits * 4);
-  pl.off_s = take(N * pl.splits * 4);
+  pl.off_m = take(N * pl.pieces * 4);
+  pl.off_s = take(N * pl.pieces * 4);
   pl.off_ent = take(N * 4);
   pl.off_mass = take(N * 4);
   pl.off_part = take(pl.blocks * 8);
@@ -454,13 +525,6 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t K) {
   return pl;
 }
 
-template <int KIND>
-struct Cfgs {
-  using Z = TileCfg<KIND, false, false, 256, true, 8>;   // dz = H W^T
-  using H = TileCfg<KIND, false, true, 256, true, 8>;    // dh = dz W
-  using W = TileCfg<KIND, true, true, 256, true, 8>;     // dW = dz^T H
-};
-
 int sum_splits(const float* part, int splits, int64_t split_elems, int64_t n, void* out, int dtype, cudaStream_t s) {
   const int64_t n4 = n / 4;  // K is a multiple of 8
   const int blocks = (int)std::min<int64_t>((n4 + 255) / 256, int64_t(get_sm_count()) * 8);
@@ -492,6 +556,7 @@ int grad_product(const CUtensorMap& a, const CUtensorMap& b, int64_t rows, int64
   prm.N = (int)K;
   prm.n_k = (int)stages;
   prm.k_per_split = (prm.n_k + splits - 1) / splits;
+  prm.per_unit = 0;
   prm.split_rows = split_rows;
   prm.out = out;
   prm.ld_out = K;
@@ -512,6 +577,28 @@ int grad_product_as(int dtype, const CUtensorMap& a, const CUtensorMap& b, int64
                                           grad_out, factor, status, name, s);
   return grad_product<C, __half>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows, grad_out,
                                  factor, status, name, s);
+}
+
+template <int KIND>
+int run_stats(const void* hidden, const void* weight, int64_t N, int64_t V, int64_t K, const StatsEpilogue& ep,
+              uint32_t* status, cudaStream_t s) {
+  using Z = typename Cfgs<KIND>::Z;
+  TileParams<StatsEpilogue> prm;
+  int st = tile_operand_map<Z>(&prm.tm_a, hidden, false, N, K, K, 128);
+  if (st != MT_OK) return st;
+  if ((st = tile_operand_map<Z>(&prm.tm_b, weight, false, V, K, K, Z::B_ROWS)) != MT_OK) return st;
+  prm.tm_out = prm.tm_a;  // not used
+  prm.M = (int)N;
+  prm.N = (int)V;
+  prm.n_k = (int)((K + Z::BK - 1) / Z::BK);
+  prm.k_per_split = prm.n_k;
+  prm.per_unit = ep.per_unit;
+  prm.split_rows = 0;
+  prm.out = nullptr;
+  prm.ld_out = 0;
+  prm.status = status;
+  prm.ep = ep;
+  return launch_tile_gemm<Z>(prm, 1, "distill_stats", s);
 }
 
 struct BwdArgs {
@@ -557,6 +644,7 @@ int run_bwd(const BwdArgs& a, const BwdPlan& pl) {
     zp.N = (int)a.V;
     zp.n_k = (int)((a.K + Z::BK - 1) / Z::BK);
     zp.k_per_split = zp.n_k;
+    zp.per_unit = 0;
     zp.split_rows = 0;
     zp.out = dz;
     zp.ld_out = pl.ld;
@@ -669,14 +757,14 @@ extern "C" int mt_distill_fwd(const void* hidden, const void* weight, int dtype,
   else
     distill_prep_kernel<__half><<<blocks, 256, 0, s>>>(pp);
   if ((st = check_launch("distill_prep")) != MT_OK) return st;
-  if ((st = logit_stats(hidden, weight, dtype, N, V, K, kLog2e / temperature, pl.splits, pm, ps, status, s)) != MT_OK)
-    return st;
-  const RowParams rp{hidden, weight, (int)N, (int)K, (int)top, pl.splits, pm, ps, list_ids, list_probs, ent, mass,
-                     1.f / temperature, list_logits, row_stats, part};
-  if (dtype == MT_BF16)
-    distill_row_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(rp);
-  else
-    distill_row_kernel<__half><<<blocks, 256, 0, s>>>(rp);
+  const StatsEpilogue ep{list_ids, list_logits, pm, ps, (int)V, (int)top, pl.pieces, kGroups, pl.n_nt, pl.per_unit,
+                         kLog2e / temperature};
+  st = dtype == MT_BF16 ? run_stats<kKindBf16>(hidden, weight, N, V, K, ep, status, s)
+                        : run_stats<kKindF16>(hidden, weight, N, V, K, ep, status, s);
+  if (st != MT_OK) return st;
+  const RowParams rp{(int)N, (int)top, pl.pieces, kGroups, pl.n_nt, pl.per_unit, pm, ps, list_ids, list_probs,
+                     list_logits, ent, mass, 1.f / temperature, row_stats, part};
+  distill_row_kernel<<<blocks, 256, 0, s>>>(rp);
   if ((st = check_launch("distill_row")) != MT_OK) return st;
   distill_loss_kernel<<<1, 1024, 0, s>>>(part, (int)pl.blocks, temperature, row_stats + N, loss);
   return check_launch("distill_loss");

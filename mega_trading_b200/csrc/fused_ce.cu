@@ -28,7 +28,6 @@
 #include <type_traits>
 
 #include "common.cuh"
-#include "fused_ce.cuh"
 
 namespace mt {
 namespace {
@@ -64,7 +63,6 @@ struct CeParams {
   float* part_s;
   float* part_z;
   int splits;
-  float zscale;  // STATS: log2(e) / temperature
   uint32_t* status;
 };
 
@@ -72,8 +70,7 @@ __device__ __forceinline__ int64_t load_label(const CeParams& p, int row) {
   return p.labels_i64 ? static_cast<const int64_t*>(p.labels)[row] : (int64_t) static_cast<const int32_t*>(p.labels)[row];
 }
 
-// STATS: no labels; row statistics of the logits times a caller's scale (part_m, part_s only).
-template <typename T, bool STATS>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_constant__ CeParams p) {
   using C = CeCfg;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -184,12 +181,12 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
     const int r = threadIdx.x & 127;   // row within the tile = TMEM lane
     const int row = row0 + r;
     const bool in_rows = row < p.N;
-    const int64_t label = !STATS && in_rows ? load_label(p, row) : p.ignore_index;
-    const bool valid = !STATS && in_rows && label != p.ignore_index && label >= 0 && label < p.V;
-    if (!STATS && wg == 0 && in_rows && label != p.ignore_index && (label < 0 || label >= p.V))
+    const int64_t label = in_rows ? load_label(p, row) : p.ignore_index;
+    const bool valid = in_rows && label != p.ignore_index && label >= 0 && label < p.V;
+    if (wg == 0 && in_rows && label != p.ignore_index && (label < 0 || label >= p.V))
       atomicCAS(p.status, 0u, (kKernelId << 16) | 0xEEEEu);  // out-of-range target
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
-    const float kLog2e = STATS ? p.zscale : 1.4426950408889634f;
+    constexpr float kLog2e = 1.4426950408889634f;
     float m = -INFINITY, s = 0.f, zy = NAN;
     bool ok = true;
     for (int t = 0; t < n_vt; ++t) {
@@ -248,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_logits_kernel(const __grid_con
         const int64_t idx = int64_t(row) * p.splits + split;
         p.part_m[idx] = mn;
         p.part_s[idx] = sm;
-        if constexpr (!STATS) p.part_z[idx] = zm;
+        p.part_z[idx] = zm;
       }
     }
   }
@@ -379,10 +376,10 @@ int ce_validate(const void* hidden, const void* weight, const void* labels, int 
   return MT_OK;
 }
 
-template <typename T, bool STATS>
+template <typename T>
 int launch_logits(const CeParams& prm, int64_t N, cudaStream_t stream) {
   using C = CeCfg;
-  auto kern = ce_logits_kernel<T, STATS>;
+  auto kern = ce_logits_kernel<T>;
   int st = set_smem_limit((const void*)kern, C::SMEM);
   if (st != MT_OK) return st;
   dim3 grid((unsigned)((N + kBM - 1) / kBM), (unsigned)prm.splits);
@@ -391,32 +388,6 @@ int launch_logits(const CeParams& prm, int64_t N, cudaStream_t stream) {
 }
 
 }  // namespace
-
-int logit_stats_splits(int64_t N, int64_t V) { return ce_splits(N, V); }
-
-int logit_stats(const void* hidden, const void* weight, int dtype, int64_t N, int64_t V, int64_t K, float zscale,
-                int splits, float* part_m, float* part_s, uint32_t* status, cudaStream_t stream) {
-  CeParams prm;
-  int st = ce_maps(prm, hidden, weight, dtype, N, V, K);
-  if (st != MT_OK) return st;
-  prm.labels = nullptr;
-  prm.labels_i64 = 0;
-  prm.ignore_index = 0;
-  prm.N = (int)N;
-  prm.V = (int)V;
-  prm.K = (int)K;
-  prm.n_vtiles = (int)((V + kBN - 1) / kBN);
-  prm.splits = splits;
-  prm.tiles_per_split = (prm.n_vtiles + splits - 1) / splits;
-  prm.part_m = part_m;
-  prm.part_s = part_s;
-  prm.part_z = nullptr;
-  prm.zscale = zscale;
-  prm.status = status;
-  return dtype == MT_BF16 ? launch_logits<__nv_bfloat16, true>(prm, N, stream)
-                          : launch_logits<__half, true>(prm, N, stream);
-}
-
 }  // namespace mt
 
 using namespace mt;
@@ -460,7 +431,7 @@ extern "C" int mt_fused_ce_fwd(const void* hidden, const void* weight, const voi
   prm.part_s = ws.ps;
   prm.part_z = ws.pz;
   prm.status = status;
-  st = dtype == MT_BF16 ? launch_logits<__nv_bfloat16, false>(prm, N, s) : launch_logits<__half, false>(prm, N, s);
+  st = dtype == MT_BF16 ? launch_logits<__nv_bfloat16>(prm, N, s) : launch_logits<__half>(prm, N, s);
   if (st != MT_OK) return st;
   ce_merge_kernel<<<(unsigned)((N + 255) / 256), 256, 0, s>>>(ws.pm, ws.ps, ws.pz, splits, (int)N, labels, labels_i64,
                                                                ignore_index, (int)V, ws.lse2, ws.row_loss,

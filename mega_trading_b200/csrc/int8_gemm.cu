@@ -22,6 +22,7 @@ template <typename TO>
 struct Int8Epilogue {
   static constexpr uint32_t kKernelId = mt::kKernelId;
   static constexpr int OUT_SIZE = sizeof(TO);
+  static constexpr bool kStats = false;
   const float* xs;
   const float* ws;
   int n;
@@ -126,6 +127,7 @@ int launch_tiles(const int8_t* x, const float* xs, const int8_t* w, const float*
   prm.N = N;
   prm.n_k = (K + C::BK - 1) / C::BK;
   prm.k_per_split = prm.n_k;
+  prm.per_unit = 0;
   prm.split_rows = 0;
   prm.out = y;
   prm.ld_out = N;

@@ -132,6 +132,7 @@ struct TileParams {
   int M, N;                  // output rows and columns
   int n_mt, n_nt, n_tiles;   // n_tiles = n_mt * n_nt * splits, columns fastest, splits slowest
   int n_k, k_per_split;      // stages of K in total and per split
+  int per_unit;              // > 0: a CTA (pair) takes this many consecutive tiles; 0: every n-th
   int64_t split_rows;        // rows of the output map between two splits
   void* out;                 // direct stores only
   int64_t ld_out;
@@ -141,6 +142,16 @@ struct TileParams {
 
 // byte offset of 16-byte chunk j of row r in a 128-byte-swizzled box
 __device__ __forceinline__ int box128_off(int r, int j) { return r * 128 + ((j ^ (r & 7)) << 4); }
+
+// One 32-bit TMEM column of the warp's 32 lanes.
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+  uint32_t v;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(v)
+               : "r"(taddr)
+               : "memory");
+  return v;
+}
 
 // Element-wise fp32 add of a staging box into global memory.
 __device__ __forceinline__ void tma_out(const CUtensorMap* map, const void* src, int c0, int c1, bool add) {
@@ -161,6 +172,15 @@ __device__ __forceinline__ void tma_out(const CUtensorMap* map, const void* src,
 //       32 accumulator columns and their column values (shared memory) -> 16
 //       (OUT_SIZE 2) or 32 (4) packed words
 //   bool add, direct                        TMA add instead of store; plain stores
+// or, with `static constexpr bool kStats = true` (per_unit > 0), nothing is
+// written per tile and a thread keeps its row's state over consecutive tiles:
+//   struct State;
+//   void begin(State&, int m, bool live, int mt, int unit, int group)
+//   int next(const State&)                  next column whose value is asked for
+//   void take(State&, uint32_t z)           gets it and moves on
+//   void skip(State&)                       moves on without it
+//   void add(State&, const uint32_t (&z)[32], int n0)
+//   void end(const State&)                  the row's last tile of this CTA is done
 template <class C, class EP>
 __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_constant__ TileParams<EP> p) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -187,6 +207,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
   const int n_units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
   const int row_off = (int)rank * 128;
   const int per_split = p.n_mt * p.n_nt;
+  const int t_begin = p.per_unit > 0 ? unit * p.per_unit : unit;
+  const int t_end = p.per_unit > 0 ? min(t_begin + p.per_unit, p.n_tiles) : p.n_tiles;
+  const int t_step = p.per_unit > 0 ? 1 : n_units;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::NST; ++s) {
@@ -222,13 +245,13 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
     return wait_bounded_long<PAIR>(wc, bar, parity, site);
   };
   struct Tile {
-    int m0, n0, k0, k1, split;
+    int m0, n0, k0, k1, split, mt;
   };
   auto tile_at = [&](int t) {
     const int split = t / per_split, u = t - split * per_split;
     const int mt = u / p.n_nt, nt = u - mt * p.n_nt;
     const int k0 = split * p.k_per_split;
-    return Tile{mt * C::TM + row_off, nt * C::BN, k0, min(k0 + p.k_per_split, p.n_k), split};
+    return Tile{mt * C::TM + row_off, nt * C::BN, k0, min(k0 + p.k_per_split, p.n_k), split, mt};
   };
 
   if (warp == C::EW) {
@@ -238,7 +261,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
       tma_prefetch_desc(&p.tm_b);
       int it = 0;
       bool ok = true;
-      for (int t = unit; ok && t < p.n_tiles; t += n_units) {
+      for (int t = t_begin; ok && t < t_end; t += t_step) {
         const Tile w = tile_at(t);
         const int b0 = w.n0 + (int)rank * C::B_ROWS;
         for (int kc = w.k0; kc < w.k1; ++kc, ++it) {
@@ -294,7 +317,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
       const uint32_t base = smem_u32(smem);
       int it = 0, lt = 0;
       bool ok = true;
-      for (int t = unit; ok && t < p.n_tiles; t += n_units, ++lt) {
+      for (int t = t_begin; ok && t < t_end; t += t_step, ++lt) {
         const Tile w = tile_at(t);
         const int buf = lt & 1;
         if (lt >= 2 && !wait_x(&acc_empty[buf], ((lt >> 1) & 1) ^ 1, 2)) break;
@@ -346,92 +369,133 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    constexpr int kCols = 128 / EP::OUT_SIZE;  // columns of a step
-    constexpr int kSub = kCols / 32;
-    constexpr int kSteps = C::BN / kCols;
     constexpr int kGroups = C::EW / 4;
-    const int wg = warp >> 2;         // takes the column steps c with c % kGroups == wg
+    const int wg = warp >> 2;
     const int r = threadIdx.x & 127;  // row within the tile = TMEM lane
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
-    uint8_t* box = smem + C::OFF_OUT + warp * C::BOX;
-    float* cols = reinterpret_cast<float*>(smem + C::OFF_COL) + warp * 64;
     const uint32_t acc_empty_x[2] = {PAIR ? cluster_addr(&acc_empty[0], 0) : 0u,
                                      PAIR ? cluster_addr(&acc_empty[1], 0) : 0u};
-    int lt = 0;
-    for (int t = unit; t < p.n_tiles; t += n_units, ++lt) {
-      const Tile w = tile_at(t);
-      const int buf = lt & 1;
-      const int m = w.m0 + r;
-      const auto rv = p.ep.row(m, m < p.M);
-      auto fetch_cols = [&](int c) {
-        // this step's per-column values, one or two per lane
-        if constexpr (EP::kCols) {
-          __syncwarp();
-#pragma unroll
-          for (int h = 0; h < kSub; ++h) cols[h * 32 + lane] = p.ep.col(w.n0 + c * kCols + h * 32 + lane);
-          __syncwarp();
+    auto release = [&](int buf) {
+      // this warp's last read of the accumulator
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR)
+          mbar_arrive_remote(acc_empty_x[buf]);
+        else
+          mbar_arrive(&acc_empty[buf]);
+      }
+    };
+    if constexpr (EP::kStats) {
+      // a warpgroup takes BN / kGroups consecutive columns of every tile
+      constexpr int kSpan = C::BN / kGroups;
+      typename EP::State st;
+      int lt = 0, mt = -1;
+      for (int t = t_begin; t < t_end; t += t_step, ++lt) {
+        const Tile w = tile_at(t);
+        const int buf = lt & 1;
+        if (w.mt != mt) {
+          if (mt >= 0) p.ep.end(st);
+          mt = w.mt;
+          p.ep.begin(st, w.m0 + r, w.m0 + r < p.M, mt, unit, wg);
         }
-      };
-      if (wg < kSteps) fetch_cols(wg);
-      if (!__all_sync(0xffffffffu, wait_x(&acc_full[buf], (lt >> 1) & 1, 8))) break;
-      tc_fence_after();
-      const uint32_t acc = tmem + lane_off + buf * C::BN;
-      const int warp_row = w.m0 + (warp & 3) * 32;
-      auto release = [&]() {
-        // this warp's last read of the accumulator
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR)
-            mbar_arrive_remote(acc_empty_x[buf]);
-          else
-            mbar_arrive(&acc_empty[buf]);
-        }
-      };
-      if (wg >= kSteps) release();
+        if (!__all_sync(0xffffffffu, wait_x(&acc_full[buf], (lt >> 1) & 1, 8))) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + lane_off + buf * C::BN;
 #pragma unroll 1
-      for (int c = wg; c < kSteps; c += kGroups) {
-        uint32_t z[kSub][32];
-#pragma unroll
-        for (int h = 0; h < kSub; ++h) tmem_ld32(acc + c * kCols + h * 32, z[h]);
-        tmem_ld_wait();
-        if (c + kGroups >= kSteps) release();
-        const int n0 = w.n0 + c * kCols;
-        if (n0 >= p.N) continue;  // nothing of this step exists (warp-uniform)
-        if (c != wg) fetch_cols(c);
-        uint32_t words[32];
-#pragma unroll
-        for (int h = 0; h < kSub; ++h) p.ep.pack(z[h], rv, cols + h * 32, words + h * 16);
-        if (lane == 0) bulk_wait_group_read0();  // the box's previous store has left it
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          *reinterpret_cast<uint4*>(box + box128_off(lane, j)) =
-              make_uint4(words[4 * j], words[4 * j + 1], words[4 * j + 2], words[4 * j + 3]);
-        if (p.ep.direct) {
-          __syncwarp();
-          using W = typename std::conditional<EP::OUT_SIZE == 2, uint16_t, uint32_t>::type;
-          const int rows = min(32, p.M - warp_row);
-          for (int i = 0; i < rows; ++i) {
-            W* dst = static_cast<W*>(p.out) + (w.split * p.split_rows + warp_row + i) * p.ld_out + n0;
-#pragma unroll
-            for (int e = lane; e < kCols; e += 32)
-              if (n0 + e < p.N)
-                dst[e] = *reinterpret_cast<const W*>(box + box128_off(i, e * EP::OUT_SIZE / 16) +
-                                                     (e * EP::OUT_SIZE) % 16);
+        for (int c = wg * kSpan; c < (wg + 1) * kSpan; c += 32) {
+          uint32_t z[32];
+          tmem_ld32(acc + c, z);
+          tmem_ld_wait();
+          const int n0 = w.n0 + c;
+          while (__any_sync(0xffffffffu, p.ep.next(st) < n0))
+            if (p.ep.next(st) < n0) p.ep.skip(st);
+          while (true) {
+            // one asked-for column at a time, read again out of TMEM (registers cannot be indexed)
+            const int want = p.ep.next(st);
+            const uint32_t asking = __ballot_sync(0xffffffffu, want < n0 + 32);
+            if (asking == 0) break;
+            const int col = __shfl_sync(0xffffffffu, want, __ffs(asking) - 1);
+            const uint32_t v = tmem_ld1(acc + (col - w.n0));
+            if (want == col) p.ep.take(st, v);
           }
+          if (c + 32 >= (wg + 1) * kSpan) release(buf);
+          p.ep.add(st, z, n0);
+        }
+      }
+      if (mt >= 0) p.ep.end(st);
+    } else {
+      constexpr int kCols = 128 / EP::OUT_SIZE;  // columns of a step
+      constexpr int kSub = kCols / 32;
+      constexpr int kSteps = C::BN / kCols;
+      // a warpgroup takes the column steps c with c % kGroups == wg
+      uint8_t* box = smem + C::OFF_OUT + warp * C::BOX;
+      float* cols = reinterpret_cast<float*>(smem + C::OFF_COL) + warp * 64;
+      int lt = 0;
+      for (int t = t_begin; t < t_end; t += t_step, ++lt) {
+        const Tile w = tile_at(t);
+        const int buf = lt & 1;
+        const int m = w.m0 + r;
+        const auto rv = p.ep.row(m, m < p.M);
+        auto fetch_cols = [&](int c) {
+          // this step's per-column values, one or two per lane
+          if constexpr (EP::kCols) {
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < kSub; ++h) cols[h * 32 + lane] = p.ep.col(w.n0 + c * kCols + h * 32 + lane);
+            __syncwarp();
+          }
+        };
+        if (wg < kSteps) fetch_cols(wg);
+        if (!__all_sync(0xffffffffu, wait_x(&acc_full[buf], (lt >> 1) & 1, 8))) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + lane_off + buf * C::BN;
+        const int warp_row = w.m0 + (warp & 3) * 32;
+        if (wg >= kSteps) release(buf);
+#pragma unroll 1
+        for (int c = wg; c < kSteps; c += kGroups) {
+          uint32_t z[kSub][32];
+#pragma unroll
+          for (int h = 0; h < kSub; ++h) tmem_ld32(acc + c * kCols + h * 32, z[h]);
+          tmem_ld_wait();
+          if (c + kGroups >= kSteps) release(buf);
+          const int n0 = w.n0 + c * kCols;
+          if (n0 >= p.N) continue;  // nothing of this step exists (warp-uniform)
+          if (c != wg) fetch_cols(c);
+          uint32_t words[32];
+#pragma unroll
+          for (int h = 0; h < kSub; ++h) p.ep.pack(z[h], rv, cols + h * 32, words + h * 16);
+          if (lane == 0) bulk_wait_group_read0();  // the box's previous store has left it
           __syncwarp();
-        } else {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_out(&p.tm_out, box, n0, (int)(w.split * p.split_rows) + warp_row, p.ep.add);
-            bulk_commit_group();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(box + box128_off(lane, j)) =
+                make_uint4(words[4 * j], words[4 * j + 1], words[4 * j + 2], words[4 * j + 3]);
+          if (p.ep.direct) {
+            __syncwarp();
+            using W = typename std::conditional<EP::OUT_SIZE == 2, uint16_t, uint32_t>::type;
+            const int rows = min(32, p.M - warp_row);
+            for (int i = 0; i < rows; ++i) {
+              W* dst = static_cast<W*>(p.out) + (w.split * p.split_rows + warp_row + i) * p.ld_out + n0;
+#pragma unroll
+              for (int e = lane; e < kCols; e += 32)
+                if (n0 + e < p.N)
+                  dst[e] = *reinterpret_cast<const W*>(box + box128_off(i, e * EP::OUT_SIZE / 16) +
+                                                       (e * EP::OUT_SIZE) % 16);
+            }
+            __syncwarp();
+          } else {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_out(&p.tm_out, box, n0, (int)(w.split * p.split_rows) + warp_row, p.ep.add);
+              bulk_commit_group();
+            }
           }
         }
       }
+      if (lane == 0) bulk_wait_group0();  // stores done before the CTA exits
     }
-    if (lane == 0) bulk_wait_group0();  // stores done before the CTA exits
   }
 
   __syncwarp();
@@ -483,13 +547,15 @@ inline int tile_output_map(CUtensorMap* m, void* base, int dtype, int64_t rows, 
 
 template <class C, class EP>
 int launch_tile_gemm(TileParams<EP>& prm, int splits, const char* name, cudaStream_t stream) {
+  static_assert(std::is_trivially_copyable<EP>::value, "kernel parameter");
   prm.n_mt = (prm.M + C::TM - 1) / C::TM;
   prm.n_nt = (prm.N + C::BN - 1) / C::BN;
   const int64_t tiles = int64_t(prm.n_mt) * prm.n_nt * splits;
   if (tiles > 0x7fffffffLL) return MT_ERR_INVALID_ARGUMENT;
   prm.n_tiles = (int)tiles;
   constexpr int per_unit = C::PAIR ? 2 : 1;
-  const int units = (int)std::min<int64_t>(tiles, get_sm_count() / per_unit);
+  int units = (int)std::min<int64_t>(tiles, get_sm_count() / per_unit);
+  if (prm.per_unit > 0) units = (int)((tiles + prm.per_unit - 1) / prm.per_unit);
   auto kern = tile_gemm_kernel<C, EP>;
   int st = set_smem_limit((const void*)kern, C::SMEM);
   if (st != MT_OK) return st;
