@@ -59,17 +59,16 @@ struct PrepParams {
   uint32_t* status;
 };
 
-// One warp per row.
-template <typename TL>
+// One warp per row, kPer list entries per lane.
+template <typename TL, int kPer>
 __global__ void __launch_bounds__(256) distill_prep_kernel(const PrepParams p) {
-  __shared__ int s_id[8][kMaxTop];
-  __shared__ int o_id[8][kMaxTop];
-  __shared__ float o_p[8][kMaxTop];
+  __shared__ int s_id[8][kPer * 32];
+  __shared__ int o_id[8][kPer * 32];
+  __shared__ float o_p[8][kPer * 32];
   const int lane = lane_id(), w = warp_id();
   const int64_t row = int64_t(blockIdx.x) * 8 + w;
   if (row >= p.N) return;
   const int top = p.top;
-  constexpr int kPer = kMaxTop / 32;
   float a[kPer];
   int id[kPer];
   float mx = -INFINITY;
@@ -238,7 +237,6 @@ struct RowParams {
   int N, top, pieces, groups, n_nt, per_unit;
   const float* part_m;
   const float* part_s;
-  const int* tid;
   const float* tp;
   const float* zt;
   const float* ent;
@@ -271,8 +269,8 @@ __global__ void __launch_bounds__(256) distill_row_kernel(const RowParams p) {
       float cross = 0.f;
       for (int j = lane; j < p.top; j += 32) {
         const int64_t at = row * p.top + j;
-        const float pr = p.tp[at];
-        if (p.tid[at] != kNone && pr != 0.f) cross += pr * (p.zt[at] * p.inv_temp - l2 * kLn2);
+        const float pr = p.tp[at];  // 0 past the list's end
+        if (pr != 0.f) cross += pr * (p.zt[at] * p.inv_temp - l2 * kLn2);
       }
       loss = p.ent[row] - warp_sum(cross);
       count = 1.f;
@@ -424,13 +422,15 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict
 // ---------------------------------------------------------------------------
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
+constexpr int kStatsWarps = 16;
+constexpr int kGroups = kStatsWarps / 4;  // warpgroups that share a row's statistics
 template <int KIND>
 struct Cfgs {
-  using Z = TileCfg<KIND, false, false, 256, true, 8>;   // H W^T: statistics, dz
+  using S = TileCfg<KIND, false, false, 256, true, kStatsWarps>;  // row statistics of H W^T
+  using Z = TileCfg<KIND, false, false, 256, true, 8>;   // dz from H W^T
   using H = TileCfg<KIND, false, true, 256, true, 8>;    // dh = dz W
   using W = TileCfg<KIND, true, true, 256, true, 8>;     // dW = dz^T H
 };
-constexpr int kGroups = 2;  // warpgroups of 8 epilogue warps
 
 struct FwdPlan {
   int n_nt, per_unit, pieces;
@@ -487,12 +487,12 @@ int choose_k_splits(int64_t tiles, int64_t k_stages) {
   return even_splits(k_stages, best);
 }
 
-constexpr int64_t kDzBytes = int64_t(512) << 20;  // most of the workspace: one chunk's dz
+constexpr int64_t kDzBytes = int64_t(256) << 20;  // most of the workspace: one chunk's dz
 
 struct BwdPlan {
   int64_t ld;          // dz row stride (elements)
   int64_t rows;        // rows per chunk
-  int chunks, h_splits, w_splits;
+  int chunks, h_splits, h_last, w_splits;
   int64_t h_pad, w_pad;  // rows of one split's partials
   int64_t off_dz, off_h, off_w, bytes;
 };
@@ -508,6 +508,9 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t K) {
   pl.chunks = (int)((N + pl.rows - 1) / pl.rows);
   const int64_t h_tiles = (pl.rows + 255) / 256 * nt, w_tiles = (V + 255) / 256 * nt;
   pl.h_splits = choose_k_splits(h_tiles, (V + 63) / 64);
+  // a shorter last chunk has fewer tiles and takes more splits
+  const int64_t last = N - (pl.chunks - 1) * pl.rows;
+  pl.h_last = choose_k_splits((last + 255) / 256 * nt, (V + 63) / 64);
   pl.w_splits = choose_k_splits(w_tiles, (pl.rows + 63) / 64);
   pl.h_pad = (pl.rows + 255) / 256 * 256;
   pl.w_pad = (V + 255) / 256 * 256;
@@ -518,7 +521,9 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t K) {
     return o;
   };
   pl.off_dz = take(pl.rows * pl.ld * 2);
-  pl.off_h = take(pl.h_splits > 1 ? pl.h_splits * pl.h_pad * K * 4 : 0);
+  const int64_t last_pad = (last + 255) / 256 * 256;
+  pl.off_h = take(std::max(pl.h_splits > 1 ? pl.h_splits * pl.h_pad : 0,
+                           pl.h_last > 1 ? pl.h_last * last_pad : 0) * K * 4);
   // fp32 sums of dW: several splits, or several chunks of a 16-bit gradient
   pl.off_w = take(pl.w_splits * pl.w_pad * K * 4);
   pl.bytes = at;
@@ -527,7 +532,7 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t K) {
 
 int sum_splits(const float* part, int splits, int64_t split_elems, int64_t n, void* out, int dtype, cudaStream_t s) {
   const int64_t n4 = n / 4;  // K is a multiple of 8
-  const int blocks = (int)std::min<int64_t>((n4 + 255) / 256, int64_t(get_sm_count()) * 8);
+  const int blocks = (int)std::min<int64_t>((n4 + 255) / 256, int64_t(get_sm_count()) * 64);
   if (dtype == MT_F32)
     sum_splits_kernel<float><<<blocks, 256, 0, s>>>(part, splits, split_elems, n4, static_cast<float*>(out));
   else if (dtype == MT_BF16)
@@ -579,18 +584,29 @@ int grad_product_as(int dtype, const CUtensorMap& a, const CUtensorMap& b, int64
                                  factor, status, name, s);
 }
 
+template <typename TL>
+int launch_prep(const PrepParams& p, unsigned blocks, cudaStream_t s) {
+  if (p.top <= 32)
+    distill_prep_kernel<TL, 1><<<blocks, 256, 0, s>>>(p);
+  else if (p.top <= 64)
+    distill_prep_kernel<TL, 2><<<blocks, 256, 0, s>>>(p);
+  else
+    distill_prep_kernel<TL, kMaxTop / 32><<<blocks, 256, 0, s>>>(p);
+  return check_launch("distill_prep");
+}
+
 template <int KIND>
 int run_stats(const void* hidden, const void* weight, int64_t N, int64_t V, int64_t K, const StatsEpilogue& ep,
               uint32_t* status, cudaStream_t s) {
-  using Z = typename Cfgs<KIND>::Z;
+  using C = typename Cfgs<KIND>::S;
   TileParams<StatsEpilogue> prm;
-  int st = tile_operand_map<Z>(&prm.tm_a, hidden, false, N, K, K, 128);
+  int st = tile_operand_map<C>(&prm.tm_a, hidden, false, N, K, K, 128);
   if (st != MT_OK) return st;
-  if ((st = tile_operand_map<Z>(&prm.tm_b, weight, false, V, K, K, Z::B_ROWS)) != MT_OK) return st;
+  if ((st = tile_operand_map<C>(&prm.tm_b, weight, false, V, K, K, C::B_ROWS)) != MT_OK) return st;
   prm.tm_out = prm.tm_a;  // not used
   prm.M = (int)N;
   prm.N = (int)V;
-  prm.n_k = (int)((K + Z::BK - 1) / Z::BK);
+  prm.n_k = (int)((K + C::BK - 1) / C::BK);
   prm.k_per_split = prm.n_k;
   prm.per_unit = ep.per_unit;
   prm.split_rows = 0;
@@ -598,7 +614,7 @@ int run_stats(const void* hidden, const void* weight, int64_t N, int64_t V, int6
   prm.ld_out = 0;
   prm.status = status;
   prm.ep = ep;
-  return launch_tile_gemm<Z>(prm, 1, "distill_stats", s);
+  return launch_tile_gemm<C>(prm, 1, "distill_stats", s);
 }
 
 struct BwdArgs {
@@ -663,12 +679,13 @@ int run_bwd(const BwdArgs& a, const BwdPlan& pl) {
       CUtensorMap ma, mb;
       if ((st = tile_operand_map<H>(&ma, dz, false, rows, a.V, pl.ld, 128)) != MT_OK) return st;
       if ((st = tile_operand_map<H>(&mb, a.weight, true, a.K, a.V, a.K, 0)) != MT_OK) return st;
-      if (pl.h_splits > 1) {
-        if ((st = grad_product_as<H>(MT_F32, ma, mb, rows, a.K, a.V, pl.h_splits, pl.h_pad, h_part, false, a.inv_rows,
+      const int splits = c + 1 == pl.chunks ? pl.h_last : pl.h_splits;
+      if (splits > 1) {
+        const int64_t pad = (rows + 255) / 256 * 256;
+        if ((st = grad_product_as<H>(MT_F32, ma, mb, rows, a.K, a.V, splits, pad, h_part, false, a.inv_rows,
                                      a.grad_out, factor, a.status, "distill_bwd_dh", a.s)) != MT_OK)
           return st;
-        if ((st = sum_splits(h_part, pl.h_splits, pl.h_pad * a.K, rows * a.K, out, a.dh_dtype, a.s)) != MT_OK)
-          return st;
+        if ((st = sum_splits(h_part, splits, pad * a.K, rows * a.K, out, a.dh_dtype, a.s)) != MT_OK) return st;
       } else if ((st = grad_product_as<H>(a.dh_dtype, ma, mb, rows, a.K, a.V, 1, 0, out, false, a.inv_rows,
                                           a.grad_out, factor, a.status, "distill_bwd_dh", a.s)) != MT_OK) {
         return st;
@@ -750,20 +767,17 @@ extern "C" int mt_distill_fwd(const void* hidden, const void* weight, int dtype,
   const PrepParams pp{teacher_ids, ids_i64, teacher_logits, ignore_index, (int)N, (int)V, (int)top, temperature,
                       list_ids, list_probs, ent, mass, status};
   const unsigned blocks = (unsigned)pl.blocks;
-  if (logits_dtype == MT_F32)
-    distill_prep_kernel<float><<<blocks, 256, 0, s>>>(pp);
-  else if (logits_dtype == MT_BF16)
-    distill_prep_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(pp);
-  else
-    distill_prep_kernel<__half><<<blocks, 256, 0, s>>>(pp);
-  if ((st = check_launch("distill_prep")) != MT_OK) return st;
+  st = logits_dtype == MT_F32    ? launch_prep<float>(pp, blocks, s)
+       : logits_dtype == MT_BF16 ? launch_prep<__nv_bfloat16>(pp, blocks, s)
+                                 : launch_prep<__half>(pp, blocks, s);
+  if (st != MT_OK) return st;
   const StatsEpilogue ep{list_ids, list_logits, pm, ps, (int)V, (int)top, pl.pieces, kGroups, pl.n_nt, pl.per_unit,
                          kLog2e / temperature};
   st = dtype == MT_BF16 ? run_stats<kKindBf16>(hidden, weight, N, V, K, ep, status, s)
                         : run_stats<kKindF16>(hidden, weight, N, V, K, ep, status, s);
   if (st != MT_OK) return st;
-  const RowParams rp{(int)N, (int)top, pl.pieces, kGroups, pl.n_nt, pl.per_unit, pm, ps, list_ids, list_probs,
-                     list_logits, ent, mass, 1.f / temperature, row_stats, part};
+  const RowParams rp{(int)N, (int)top, pl.pieces, kGroups, pl.n_nt, pl.per_unit, pm, ps, list_probs, list_logits,
+                     ent, mass, 1.f / temperature, row_stats, part};
   distill_row_kernel<<<blocks, 256, 0, s>>>(rp);
   if ((st = check_launch("distill_row")) != MT_OK) return st;
   distill_loss_kernel<<<1, 1024, 0, s>>>(part, (int)pl.blocks, temperature, row_stats + N, loss);
@@ -797,7 +811,7 @@ extern "C" int mt_distill_bwd(const void* hidden, const void* weight, int dtype,
     return MT_ERR_INVALID_ARGUMENT;
   const BwdPlan pl = plan_bwd(N, V, K);
   if (workspace == nullptr || !aligned_to(workspace, 256) || workspace_bytes < pl.bytes) return MT_ERR_WORKSPACE;
-  if (pl.h_splits * pl.h_pad > 0x7fffffffLL || pl.w_splits * pl.w_pad > 0x7fffffffLL) return MT_ERR_INVALID_ARGUMENT;
+  if (std::max(pl.h_splits, pl.h_last) * pl.h_pad > 0x7fffffffLL || pl.w_splits * pl.w_pad > 0x7fffffffLL) return MT_ERR_INVALID_ARGUMENT;
   if ((st = bind_device_of(hidden)) != MT_OK) return st;
   if ((st = check_arch()) != MT_OK) return st;
   const BwdArgs a{hidden, weight, N, V, K, (int)top, temperature, list_ids, list_probs, list_logits, row_stats,
