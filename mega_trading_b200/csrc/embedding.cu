@@ -7,20 +7,25 @@
 // src/mega_trading/model.py:20-147), whose gradient PyTorch computes.
 //
 // Forward: bound by HBM (N * dim elements written; the table stays in L2 at
-// this model's sizes).  One warp per token, 16-byte stores.
+// this model's sizes).  One warp per token, 16-byte streaming stores.
 //
 // Gradient: bound by reading dy once.  The token ids are sorted with their
 // positions (stable least-significant-digit radix sort, 8 bits a pass, written
 // here: one block for up to 4,096 tokens, otherwise a histogram launch and one
 // scatter launch per pass), so that the rows of dy which meet in one row of dW
-// are neighbours in the sorted order.  embed_reduce_kernel cuts the sorted
-// order into chunks of equal length, so a token that makes up a large share of
-// the stream costs no more than any other: a warp walks one chunk for one slab
-// of columns and sums runs of equal ids in fp32 registers, eight rows in
-// flight.  A run that lies inside its chunk goes straight to dW; a run cut by a
-// chunk border leaves fp32 partial sums, at most two per chunk, which
-// embed_join_kernel adds up (it also zeroes the rows no token chose).  Every
-// sum has a fixed order (no atomics on values): results are the same each time.
+// are neighbours in the sorted order.  The sorted order is cut into ranges of
+// equal length, so a token that makes up a large share of the stream costs no
+// more than any other, and runs of equal ids are summed in fp32 registers:
+//   embed_reduce_bulk_kernel  two blocks per SM, one range each; a producer
+//       warp gathers whole rows with bulk copies (cp.async.bulk) into a 96 KB
+//       ring, so the loads in flight do not depend on registers or on where
+//       runs end (rows of a multiple of 16 bytes)
+//   embed_reduce_kernel       any width and alignment: a warp walks a chunk of
+//       32 or 64 positions for one slab of columns
+// A run that lies inside its range goes straight to dW; a run cut by a border
+// leaves fp32 partial sums, at most two per range, which embed_join_kernel adds
+// up (it also zeroes the rows no token chose).  Every sum has a fixed order (no
+// atomics on values): results are the same each time.
 //
 // Ids outside [0, V) read nothing: their output row is zero, they add to no
 // gradient and the status word is set.  Places holding padding_idx look up
@@ -33,7 +38,8 @@ namespace mt {
 namespace {
 
 constexpr uint32_t kKernelId = 7;
-constexpr int kSubTile = 2048;   // tokens one sort block ranks at a time (8 warps x 8 x 32)
+constexpr int kRounds = 4;       // 32-token rounds a warp ranks at a time
+constexpr int kSubTile = 8 * 32 * kRounds;  // tokens one sort block ranks at a time
 constexpr int kOneBlock = 4096;  // tokens the single-block sort takes (32 warps x 4 x 32)
 constexpr int kMaxTiles = 512;   // blocks of a sort pass (a block then takes several sub-tiles)
 
@@ -68,11 +74,16 @@ __device__ __forceinline__ void load_n(const T* p, float (&v)[E]) {
     }
   }
 }
-template <typename T, int E>
+// STREAM: written once and not read soon (leaves the cache to what is)
+template <typename T, int E, bool STREAM = false>
 __device__ __forceinline__ void store_n(T* p, const float (&v)[E]) {
   constexpr int kPer = 16 / sizeof(T);
   if constexpr (E * sizeof(T) == 8) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    const uint2 q = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    if constexpr (STREAM)
+      __stcs(reinterpret_cast<uint2*>(p), q);
+    else
+      *reinterpret_cast<uint2*>(p) = q;
   } else {
 #pragma unroll
     for (int i = 0; i < E; i += kPer) {
@@ -83,7 +94,10 @@ __device__ __forceinline__ void store_n(T* p, const float (&v)[E]) {
       else
         q = make_uint4(pack2<T>(v[i], v[i + 1]), pack2<T>(v[i + 2], v[i + 3]), pack2<T>(v[i + 4], v[i + 5]),
                        pack2<T>(v[i + 6], v[i + 7]));
-      *reinterpret_cast<uint4*>(p + i) = q;
+      if constexpr (STREAM)
+        __stcs(reinterpret_cast<uint4*>(p + i), q);
+      else
+        *reinterpret_cast<uint4*>(p + i) = q;
     }
   }
 }
@@ -110,11 +124,11 @@ struct Cols {
       }
     }
   }
-  template <typename T>
+  template <typename T, bool STREAM = false>
   static __device__ __forceinline__ void store(T* row, int c0, int dim, const float (&v)[E]) {
     const int lane = lane_id();
     if constexpr (VEC) {
-      if (c0 + lane * E < dim) store_n<T, E>(row + c0 + lane * E, v);
+      if (c0 + lane * E < dim) store_n<T, E, STREAM>(row + c0 + lane * E, v);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -151,17 +165,18 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const void* __restrict__
     return;
   }
   const TW* src = w + id * dim;
-  for (int c0 = 0; c0 < dim; c0 += 4 * C::kSlab) {
-    float v[4][E];
+  constexpr int kSlabs = 32 / E;  // slabs in flight: 1,024 columns
+  for (int c0 = 0; c0 < dim; c0 += kSlabs * C::kSlab) {
+    float v[kSlabs][E];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < kSlabs; ++s)
       if (c0 + s * C::kSlab < dim) C::load(src, c0 + s * C::kSlab, dim, v[s]);
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < kSlabs; ++s)
       if (c0 + s * C::kSlab < dim) {
 #pragma unroll
         for (int e = 0; e < E; ++e) v[s][e] *= scale;
-        C::store(row, c0 + s * C::kSlab, dim, v[s]);
+        C::template store<TO, true>(row, c0 + s * C::kSlab, dim, v[s]);
       }
   }
 }
@@ -177,13 +192,13 @@ struct SortIn {
   uint32_t* status;
 };
 
-__device__ __forceinline__ uint32_t key_of(const SortIn& in, int64_t n) {
-  const int64_t id = load_id(in.ids, in.i64, n);
-  if (id < 0 || id >= in.vocab) {
-    atomicCAS(in.status, 0u, (kKernelId << 16) | 0xEEEEu);
-    return (uint32_t)in.vocab;
-  }
-  return id == in.pad ? (uint32_t)in.vocab : (uint32_t)id;
+__device__ __forceinline__ uint32_t key_of(const SortIn& in, int64_t id) {
+  if (id < 0 || id >= in.vocab || id == in.pad) return (uint32_t)in.vocab;
+  return (uint32_t)id;
+}
+// The first kernel of a gradient also reports ids outside the vocabulary.
+__device__ __forceinline__ void report_id(const SortIn& in, int64_t id) {
+  if (id < 0 || id >= in.vocab) atomicCAS(in.status, 0u, (kKernelId << 16) | 0xEEEEu);
 }
 
 // Rank of each of the tile's items among the items of its digit (in the order
@@ -258,7 +273,9 @@ __global__ void __launch_bounds__(1024) embed_sort_small_kernel(SortIn in, int n
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     pos[i] = first + i * 32;
-    key[i] = (int)pos[i] < n_tokens ? key_of(in, pos[i]) : 0u;
+    const int64_t id = (int)pos[i] < n_tokens ? load_id(in.ids, in.i64, pos[i]) : 0;
+    key[i] = key_of(in, id);
+    report_id(in, id);
   }
   for (int shift = 0; shift < bits; shift += 8) {
 #pragma unroll
@@ -282,7 +299,7 @@ __global__ void __launch_bounds__(1024) embed_sort_small_kernel(SortIn in, int n
       for (int i = 0; i < 4; ++i)
         if (first + i * 32 < n_tokens) {
           pos[i] = pos_s[first + i * 32];
-          key[i] = key_of(in, pos[i]);
+          key[i] = key_of(in, load_id(in.ids, in.i64, pos[i]));
         }
       __syncthreads();
     }
@@ -301,11 +318,21 @@ __global__ void __launch_bounds__(256) embed_hist_kernel(SortIn in, int64_t n_to
   for (int64_t v = gid; v <= in.vocab; v += gsz) seg[v] = make_uint2(0u, 0u);
   __syncthreads();
   const int64_t lo = blockIdx.x * tile, hi = min(lo + tile, n_tokens);
-  for (int64_t i = lo + threadIdx.x; i < hi + 255; i += 256) {
-    if (i - threadIdx.x >= hi) break;
-    const uint32_t d = i < hi ? key_of(in, i) & 255u : 256u;
-    const uint32_t peers = __match_any_sync(0xffffffffu, d);
-    if (d < 256 && lane_id() == __ffs(peers) - 1) atomicAdd(&h[d], (uint32_t)__popc(peers));
+  for (int64_t s0 = lo; s0 < hi; s0 += kSubTile) {
+    int64_t id[kRounds];
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int64_t n = s0 + i * 256 + threadIdx.x;
+      id[i] = n < hi ? load_id(in.ids, in.i64, n) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const bool live = s0 + i * 256 + threadIdx.x < hi;
+      const uint32_t d = live ? key_of(in, id[i]) & 255u : 256u;
+      if (live) report_id(in, id[i]);
+      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      if (d < 256 && lane_id() == __ffs(peers) - 1) atomicAdd(&h[d], (uint32_t)__popc(peers));
+    }
   }
   __syncthreads();
   hist[int64_t(blockIdx.x) * 256 + threadIdx.x] = h[threadIdx.x];
@@ -319,51 +346,67 @@ template <bool FIRST>
 __global__ void __launch_bounds__(256) embed_scatter_kernel(SortIn in, const uint2* __restrict__ src, int64_t n_tokens,
                                                             int64_t tile, int shift, const uint32_t* __restrict__ hist,
                                                             uint32_t* __restrict__ next, uint2* __restrict__ dst) {
-  __shared__ uint32_t cnt[8][256];
+  __shared__ __align__(16) uint32_t cnt[8][256];
   __shared__ uint32_t total[256], base[256], warp_tot[8];
-  {
-    // this tile's first place for every digit
-    uint32_t before = 0, all = 0;
-    const uint32_t* col = hist + threadIdx.x;
-    const int tiles = gridDim.x, me = blockIdx.x;
-#pragma unroll 16
-    for (int b = 0; b < tiles; ++b) {
-      const uint32_t c = __ldg(col + int64_t(b) * 256);
-      all += c;
-      before += b < me ? c : 0u;
-    }
-    total[threadIdx.x] = all;
-    __syncthreads();
-    scan256(total, base, warp_tot);
-    base[threadIdx.x] += before;
-    __syncthreads();
-  }
+  // this block's items of the first sub-tile, on their way while the places are summed
   const int64_t lo = blockIdx.x * tile, hi = min(lo + tile, n_tokens);
-  for (int64_t s0 = lo; s0 < hi; s0 += kSubTile) {
-    uint32_t key[8], pos[8], digit[8], rank[8];
+  uint32_t key[kRounds], pos[kRounds];
+  auto fetch = [&](int64_t s0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t n = s0 + warp_id() * 256 + i * 32 + lane_id();
-      digit[i] = 256u;
-      if (n < hi) {
-        if constexpr (FIRST) {
-          key[i] = key_of(in, n);
-          pos[i] = (uint32_t)n;
-        } else {
-          const uint2 q = src[n];
-          key[i] = q.x;
-          pos[i] = q.y;
-        }
-        digit[i] = (key[i] >> shift) & 255u;
+    for (int i = 0; i < kRounds; ++i) {
+      const int64_t n = s0 + warp_id() * (32 * kRounds) + i * 32 + lane_id();
+      if constexpr (FIRST) {
+        key[i] = key_of(in, n < hi ? load_id(in.ids, in.i64, n) : 0);
+        pos[i] = (uint32_t)n;
+      } else {
+        const uint2 q = n < hi ? src[n] : make_uint2(0u, 0u);
+        key[i] = q.x;
+        pos[i] = q.y;
       }
     }
-    rank_tile<8, 8>(digit, rank, cnt, total);
+  };
+  fetch(lo);
+  {
+    // this tile's first place for every digit: four threads share a column of
+    // four digits, each takes every fourth tile
+    const int quad = threadIdx.x & 63, grp = threadIdx.x >> 6;
+    const uint4* col = reinterpret_cast<const uint4*>(hist) + quad;
+    const int tiles = gridDim.x, me = blockIdx.x;
+    uint4 all = make_uint4(0u, 0u, 0u, 0u), before = all;
+#pragma unroll 8
+    for (int b = grp; b < tiles; b += 4) {
+      const uint4 c = __ldg(col + int64_t(b) * 64);
+      const uint32_t m = b < me ? 0xffffffffu : 0u;
+      all.x += c.x; all.y += c.y; all.z += c.z; all.w += c.w;
+      before.x += c.x & m; before.y += c.y & m; before.z += c.z & m; before.w += c.w & m;
+    }
+    *reinterpret_cast<uint4*>(&cnt[grp][quad * 4]) = all;
+    *reinterpret_cast<uint4*>(&cnt[4 + grp][quad * 4]) = before;
+    __syncthreads();
+    const int d = threadIdx.x;
+    total[d] = cnt[0][d] + cnt[1][d] + cnt[2][d] + cnt[3][d];
+    const uint32_t mine = cnt[4][d] + cnt[5][d] + cnt[6][d] + cnt[7][d];
+    __syncthreads();
+    scan256(total, base, warp_tot);
+    base[d] += mine;
+    __syncthreads();
+  }
+  for (int64_t s0 = lo; s0 < hi; s0 += kSubTile) {
+    if (s0 > lo) fetch(s0);
+    uint32_t digit[kRounds], rank[kRounds];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kRounds; ++i) {
+      const int64_t n = s0 + warp_id() * (32 * kRounds) + i * 32 + lane_id();
+      digit[i] = n < hi ? (key[i] >> shift) & 255u : 256u;
+    }
+    rank_tile<8, kRounds>(digit, rank, cnt, total);
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i)
       if (digit[i] < 256) {
         const uint32_t at = base[digit[i]] + rank[i];
         dst[at] = make_uint2(key[i], pos[i]);
-        if (next != nullptr) atomicAdd(&next[int64_t(at / (uint32_t)tile) * 256 + ((key[i] >> (shift + 8)) & 255u)], 1u);
+        if (next != nullptr)
+          atomicAdd(&next[int64_t(at / (uint32_t)tile) * 256 + ((key[i] >> (shift + 8)) & 255u)], 1u);
       }
     __syncthreads();
     base[threadIdx.x] += total[threadIdx.x];
@@ -447,71 +490,258 @@ __global__ void __launch_bounds__(256) embed_reduce_kernel(const uint2* __restri
   }
 }
 
-// Rows no token chose become zero; runs cut by chunk borders become the sum of
-// their partial sums.  A block takes 32 ids and one slab of columns; a run of
-// more than kWide partials is shared by the block's warps.
+// The same sums for rows of a multiple of 16 bytes.  A block owns one range of
+// the sorted order for one slab of columns (up to 4 KB of a row); warps 0-7 add
+// (thread = 16 bytes of the row), warp 8 gathers.  A ring stage holds 16 KB:
+// `rp` rows with the ids they belong to.
+constexpr int kBulkStage = 16384;
+constexpr int kBulkStages = 6;
+constexpr int kBulkThreads = 9 * 32;
+constexpr int kBulkSlab = 4096;  // bytes
+enum : uint32_t { kRunStarts = 1, kRunEnds = 2, kNoRow = 4 };
+
+struct BulkSmem {
+  uint8_t ring[kBulkStages][kBulkStage];
+  uint2 meta[kBulkStages][32];  // {id, flags}
+  uint64_t full[kBulkStages], empty[kBulkStages];
+  int abort_flag;
+};
+
+// 16-byte aligned copy of `bytes` (a multiple of 16) from global to this CTA's
+// shared memory, completing on its mbarrier.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <typename TG, typename TD>
+__global__ void __launch_bounds__(kBulkThreads) embed_reduce_bulk_kernel(
+    const uint2* __restrict__ sorted, int64_t n_tokens, int64_t range, int rp, const TG* __restrict__ dy,
+    uint32_t vocab, int dim, float scale, TD* __restrict__ dw, float* __restrict__ partial, uint2* __restrict__ seg,
+    uint32_t* status) {
+  constexpr int E = 16 / sizeof(TG);
+  extern __shared__ __align__(128) uint8_t raw[];
+  BulkSmem& sm = *reinterpret_cast<BulkSmem*>(raw);
+  const int64_t lo = int64_t(blockIdx.x) * range, hi = min(lo + range, n_tokens);
+  const int c0 = blockIdx.y * (kBulkSlab / (int)sizeof(TG));
+  const int cols = min(dim - c0, kBulkSlab / (int)sizeof(TG));
+  const uint32_t bytes = cols * (uint32_t)sizeof(TG);
+  const int adders = (int)(bytes + 511) / 512;  // warps that own columns
+  const int lane = lane_id(), warp = warp_id();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBulkStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], adders);
+    }
+    sm.abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  const WaitCtx wc{status, &sm.abort_flag, kKernelId};
+  if (warp == 8) {
+    // ------------------------------------------------------------ gather
+    uint32_t prev = lo > 0 ? __ldg(&sorted[lo - 1].x) : 0xffffffffu;  // ids are below 2^31
+    uint2 mine = lo + lane < hi ? __ldg(sorted + lo + lane) : make_uint2(0xffffffffu, 0u);
+    int it = 0;
+    bool ok = true;
+    for (int64_t b0 = lo; ok && b0 < hi; b0 += 32) {
+      // the pair after this batch's last one decides where its run ends
+      uint2 later = b0 + 32 + lane < n_tokens ? __ldg(sorted + b0 + 32 + lane) : make_uint2(0xffffffffu, 0u);
+      const bool in = b0 + lane < hi;
+      uint32_t before = __shfl_up_sync(0xffffffffu, mine.x, 1);
+      if (lane == 0) before = prev;
+      uint32_t after = __shfl_down_sync(0xffffffffu, mine.x, 1);
+      const uint32_t beyond = __shfl_sync(0xffffffffu, later.x, 0);
+      if (lane == 31) after = beyond;
+      if (b0 + lane + 1 == hi && hi < n_tokens) after = __ldg(&sorted[hi].x);
+      const bool row = in && mine.x < vocab;
+      const uint32_t flags = (mine.x != before ? kRunStarts : 0u) | (mine.x != after ? kRunEnds : 0u) |
+                             (row ? 0u : kNoRow);
+      prev = __shfl_sync(0xffffffffu, mine.x, 31);
+      for (int g = 0; g < 32 && b0 + g < hi; g += rp, ++it) {
+        const int st = it % kBulkStages;
+        if (it >= kBulkStages && !wait_bounded(wc, &sm.empty[st], ((it / kBulkStages) & 1) ^ 1, 1)) {
+          ok = false;
+          break;
+        }
+        const bool here = lane >= g && lane < g + rp;
+        if (here) sm.meta[st][lane - g] = make_uint2(mine.x, flags);
+        const uint32_t n = __popc(__ballot_sync(0xffffffffu, here && row));
+        if (lane == 0) {
+          if (n > 0)
+            mbar_arrive_expect_tx(&sm.full[st], n * bytes);
+          else
+            mbar_arrive(&sm.full[st]);
+        }
+        __syncwarp();
+        if (here && row)
+          bulk_load(&sm.ring[st][(lane - g) * bytes], dy + int64_t(mine.y) * dim + c0, bytes, &sm.full[st]);
+      }
+      mine = b0 + 32 + lane < hi ? later : make_uint2(0xffffffffu, 0u);
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok || sm.abort_flag) {
+      for (int j = (it > kBulkStages ? it - kBulkStages : 0); j < it; ++j)
+        wait_drain(wc, &sm.full[j % kBulkStages], (j / kBulkStages) & 1, 11);
+    }
+  } else if (warp < adders) {
+    // ------------------------------------------------------------ add
+    const bool own = threadIdx.x * 16 < (int)bytes;
+    const int col = c0 + threadIdx.x * E;
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    bool begins = true;  // the current run begins in this range
+    int64_t at = lo;
+    for (int it = 0; at < hi; ++it) {
+      const int st = it % kBulkStages;
+      if (!wait_bounded(wc, &sm.full[st], (it / kBulkStages) & 1, 2)) break;
+      const int rows = (int)min((int64_t)rp, hi - at);
+      // four rows at a time: their values and run flags are fetched together
+      for (int i0 = 0; i0 < rows; i0 += 4) {
+        uint2 m[4];
+        uint4 q[4];
+        uint32_t any = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m[j] = sm.meta[st][i0 + j];
+          if (i0 + j >= rows) m[j].y = kNoRow;
+          any |= m[j].y;
+          q[j] = *reinterpret_cast<const uint4*>(&sm.ring[st][own ? (i0 + j) * bytes + threadIdx.x * 16 : 0]);
+        }
+        auto add = [&](const uint4& v) {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          if constexpr (sizeof(TG) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += __uint_as_float(w[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float a, b;
+              unpack2<TG>(w[e], a, b);
+              acc[2 * e] += a;
+              acc[2 * e + 1] += b;
+            }
+          }
+        };
+        if (any == 0 && at > lo && at + 4 < hi) {  // inside one run
+#pragma unroll
+          for (int j = 0; j < 4; ++j) add(q[j]);
+          at += 4;
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (i0 + j >= rows) break;
+          const int64_t here = at++;
+          if (m[j].y & kNoRow) continue;
+          if (m[j].y & kRunStarts) {
+            begins = true;
+            if (blockIdx.y == 0 && threadIdx.x == 0) seg[m[j].x].x = (uint32_t)here;
+          } else if (here == lo) {
+            begins = false;
+          }
+          add(q[j]);
+          const bool ends = m[j].y & kRunEnds;
+          if (ends && blockIdx.y == 0 && threadIdx.x == 0) seg[m[j].x].y = (uint32_t)here + 1u;
+          if (ends || here + 1 == hi) {
+            if (own) {
+              if (begins && ends) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] *= scale;
+                store_n<TD, E>(dw + int64_t(m[j].x) * dim + col, acc);
+              } else {
+                store_n<float, E>(partial + (int64_t(blockIdx.x) * 2 + (begins ? 1 : 0)) * dim + col, acc);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = 0.f;
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[st]);
+    }
+  }
+  __syncthreads();
+}
+
+// Rows no token chose become zero; runs cut by range borders become the sum of
+// their partial sums.  A warp takes 32 ids and one slab of columns; a run of
+// more than kWide partial sums is shared by the block's warps.
 template <typename TD, int E, bool VEC>
-__global__ void __launch_bounds__(256) embed_join_kernel(const uint2* __restrict__ seg, int64_t vocab, int chunk,
+__global__ void __launch_bounds__(256) embed_join_kernel(const uint2* __restrict__ seg, int64_t vocab, int64_t range,
                                                          const float* __restrict__ partial, int dim, float scale,
                                                          TD* __restrict__ dw) {
   using C = Cols<E, VEC>;
-  constexpr int kWide = 64;
+  constexpr int kWide = 16, kBatch = 32 / E;
   __shared__ float red[8][32 * E];
+  __shared__ uint32_t wide[256];
+  __shared__ int n_wide;
+  if (threadIdx.x == 0) n_wide = 0;
+  __syncthreads();
   const int c0 = blockIdx.y * C::kSlab;
   const int lane = lane_id(), w = warp_id();
-  const int64_t v0 = int64_t(blockIdx.x) * 32;
-  const uint2 mine = v0 + lane < vocab ? __ldg(seg + v0 + lane) : make_uint2(0u, 0u);
+  const int64_t v0 = int64_t(blockIdx.x) * 256 + w * 32;
+  const uint2 mine = v0 + lane < vocab ? __ldg(seg + v0 + lane) : make_uint2(0u, 1u);
+  // ranges the run touches; a run inside one range was written by the reduction
+  const int64_t a = mine.x / (uint64_t)range, b = (mine.y - (mine.y > 0 ? 1 : 0)) / (uint64_t)range;
+  const bool none = mine.x == mine.y;
+  uint32_t todo = __ballot_sync(0xffffffffu, none);
+  float zero[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) zero[e] = 0.f;
+  for (; todo != 0; todo &= todo - 1) C::store(dw + (v0 + __ffs(todo) - 1) * dim, c0, dim, zero);
+  // partial sums lo .. hi - 1 of a run whose first one is `head` (slot 1)
   auto sum = [&](int64_t lo, int64_t hi, int64_t head, float(&acc)[E]) {
-    // partials lo .. hi of a run whose first one is `head` (slot 1), eight rows in flight
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int64_t q = lo; q < hi; q += 8) {
-      float v[8][E];
+    for (int64_t q = lo; q < hi; q += kBatch) {
+      float v[kBatch][E];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < kBatch; ++j)
         if (q + j < hi) C::load(partial + ((q + j) * 2 + (q + j == head ? 1 : 0)) * dim, c0, dim, v[j]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < kBatch; ++j)
         if (q + j < hi)
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[e] += v[j][e];
     }
   };
-  for (int i = 0; i < 32; ++i) {
-    const uint32_t start = __shfl_sync(0xffffffffu, mine.x, i), end = __shfl_sync(0xffffffffu, mine.y, i);
-    if (v0 + i >= vocab) break;
-    TD* row = dw + (v0 + i) * dim;
+  const bool cut = !none && a != b;
+  if (cut && b - a >= kWide) wide[atomicAdd(&n_wide, 1)] = (uint32_t)(w * 32 + lane);
+  for (todo = __ballot_sync(0xffffffffu, cut && b - a < kWide); todo != 0; todo &= todo - 1) {
+    const int i = __ffs(todo) - 1;
+    const int64_t ra = __shfl_sync(0xffffffffu, a, i), rb = __shfl_sync(0xffffffffu, b, i);
     float acc[E];
-    if (start == end) {
-      if ((i & 7) != w) continue;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = 0.f;
-      C::store(row, c0, dim, acc);
-      continue;
-    }
-    const int64_t a = start / (uint32_t)chunk, b = (end - 1) / (uint32_t)chunk;
-    if (a == b) continue;  // written by the reduction
-    if (b - a < kWide) {
-      if ((i & 7) != w) continue;
-      sum(a, b + 1, a, acc);
-    } else {
-      const int64_t per = (b + 1 - a + 7) / 8;
-      sum(a + w * per, min(a + (w + 1) * per, b + 1), a, acc);
-#pragma unroll
-      for (int e = 0; e < E; ++e) red[w][e * 32 + lane] = acc[e];
-      __syncthreads();
-      if (w == 0) {
-#pragma unroll
-        for (int q = 1; q < 8; ++q)
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += red[q][e * 32 + lane];
-      }
-      __syncthreads();
-      if (w != 0) continue;
-    }
+    sum(ra, rb + 1, ra, acc);
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= scale;
-    C::store(row, c0, dim, acc);
+    C::store(dw + (v0 + i) * dim, c0, dim, acc);
+  }
+  __syncthreads();
+  for (int k = 0; k < n_wide; ++k) {  // in any order: each run is its own sum
+    const int64_t v = int64_t(blockIdx.x) * 256 + wide[k];
+    const uint2 run = __ldg(seg + v);
+    const int64_t ra = run.x / (uint64_t)range, rb = (run.y - 1) / (uint64_t)range;
+    const int64_t per = (rb + 1 - ra + 7) / 8;
+    float acc[E];
+    sum(ra + w * per, min(ra + (w + 1) * per, rb + 1), ra, acc);
+#pragma unroll
+    for (int e = 0; e < E; ++e) red[w][e * 32 + lane] = acc[e];
+    __syncthreads();
+    if (w == 0) {
+#pragma unroll
+      for (int q = 1; q < 8; ++q)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += red[q][e * 32 + lane];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= scale;
+      C::store(dw + v * dim, c0, dim, acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -660,17 +890,34 @@ extern "C" int mt_embedding_bwd(const void* ids, int ids_i64, int64_t n, const v
       constexpr int E = lane_elems<TG, TD>();
       const bool vec = on16(dout) && on16(dweight) && dim % E == 0 && dim % 4 == 0;
       const int slabs = (int)((dim + 32 * E - 1) / (32 * E));
-      const int64_t units = pl.chunks * slabs;
-      if ((units + 7) / 8 > 0x7fffffffLL || slabs > 65535) return (int)MT_ERR_INVALID_ARGUMENT;
-      auto red = vec ? embed_reduce_kernel<TG, TD, true> : embed_reduce_kernel<TG, TD, false>;
-      red<<<(unsigned)((units + 7) / 8), 256, 0, s>>>(sorted, n, pl.chunk, slabs, static_cast<const TG*>(dout),
-                                                      (uint32_t)vocab, (int)dim, scale, static_cast<TD*>(dweight),
-                                                      partial, seg);
-      int rc = check_launch("embedding_bwd_reduce");
-      if (rc != MT_OK) return rc;
+      int64_t range = pl.chunk;
+      int rc;
+      if (on16(dout) && on16(dweight) && (dim * sizeof(TG)) % 16 == 0) {
+        // two blocks per SM, each with an equal part of the sorted order
+        const int64_t row = dim * sizeof(TG);
+        const int64_t bslabs = (row + kBulkSlab - 1) / kBulkSlab;
+        if (bslabs > 65535) return (int)MT_ERR_INVALID_ARGUMENT;
+        const int64_t want = std::max<int64_t>(1, 2 * get_sm_count() / bslabs);
+        range = std::max<int64_t>(pl.chunk, ((n + want - 1) / want + 31) / 32 * 32);
+        int rp = 32;
+        while (rp * std::min<int64_t>(row, kBulkSlab) > kBulkStage) rp /= 2;
+        auto kern = embed_reduce_bulk_kernel<TG, TD>;
+        if ((rc = set_smem_limit((const void*)kern, sizeof(BulkSmem))) != MT_OK) return rc;
+        kern<<<dim3((unsigned)((n + range - 1) / range), (unsigned)bslabs), kBulkThreads, sizeof(BulkSmem), s>>>(
+            sorted, n, range, rp, static_cast<const TG*>(dout), (uint32_t)vocab, (int)dim, scale,
+            static_cast<TD*>(dweight), partial, seg, status);
+      } else {
+        const int64_t units = pl.chunks * slabs;
+        if ((units + 7) / 8 > 0x7fffffffLL || slabs > 65535) return (int)MT_ERR_INVALID_ARGUMENT;
+        auto red = vec ? embed_reduce_kernel<TG, TD, true> : embed_reduce_kernel<TG, TD, false>;
+        red<<<(unsigned)((units + 7) / 8), 256, 0, s>>>(sorted, n, pl.chunk, slabs, static_cast<const TG*>(dout),
+                                                        (uint32_t)vocab, (int)dim, scale, static_cast<TD*>(dweight),
+                                                        partial, seg);
+      }
+      if ((rc = check_launch("embedding_bwd_reduce")) != MT_OK) return rc;
       auto join = vec ? embed_join_kernel<TD, E, true> : embed_join_kernel<TD, E, false>;
-      join<<<dim3((unsigned)((vocab + 31) / 32), (unsigned)slabs), 256, 0, s>>>(
-          seg, vocab, pl.chunk, partial, (int)dim, scale, static_cast<TD*>(dweight));
+      join<<<dim3((unsigned)((vocab + 255) / 256), (unsigned)slabs), 256, 0, s>>>(
+          seg, vocab, range, partial, (int)dim, scale, static_cast<TD*>(dweight));
       return check_launch("embedding_bwd_join");
     });
   });
