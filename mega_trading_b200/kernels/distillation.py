@@ -29,30 +29,31 @@ class _FusedLinearDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, ids, logits, temperature, ignore_index, compute_weight):
         lib = _lib.load()
+        op = "fused_linear_distillation"
         cdtype = hidden.dtype if hidden.dtype in _COMPUTE else torch.bfloat16
-        h = _aligned(hidden.detach().to(cdtype))
-        w = _aligned((weight if compute_weight is None else compute_weight).detach().to(cdtype))
-        ids, logits = ids.contiguous(), logits.detach().contiguous()
+        h = _aligned(hidden, cdtype)
+        w = _aligned(weight if compute_weight is None else compute_weight, cdtype)
+        ids, logits = ids.contiguous(), logits.contiguous()
         n, k = h.shape
         v, top = w.shape[0], ids.shape[1]
         dev = h.device
-        loss = torch.empty((), device=dev, dtype=torch.float32)
-        list_ids = torch.empty((n, top), device=dev, dtype=torch.int32)
-        probs, z = torch.empty((2, n, top), device=dev, dtype=torch.float32).unbind(0)
-        stats = torch.empty((n + 3,), device=dev, dtype=torch.float32)
-        ws = torch.empty((int(lib.mt_distill_workspace_bytes(n, v)),), device=dev, dtype=torch.uint8)
+        loss = h.new_empty((), dtype=torch.float32)
+        # what the backward needs of the lists: ids, probabilities, logits [n, top] and the row statistics [n + 3]
+        kept = h.new_empty((3 * n * top + n + 3,), dtype=torch.float32)
+        list_ids = kept.data_ptr()
+        probs, z, stats = (list_ids + 4 * n * top * i for i in (1, 2, 3))
+        ws = h.new_empty((lib.mt_distill_workspace_bytes(n, v),), dtype=torch.uint8)
         with _lib.on_device(dev):
             st = lib.mt_distill_fwd(
                 h.data_ptr(), w.data_ptr(), _lib.dtype_code(cdtype), ids.data_ptr(),
-                1 if ids.dtype == torch.int64 else 0, ignore_index, logits.data_ptr(), _lib.dtype_code(logits.dtype),
-                n, v, k, top, temperature, loss.data_ptr(), list_ids.data_ptr(), probs.data_ptr(), z.data_ptr(),
-                stats.data_ptr(), ws.data_ptr(), ws.numel(), _lib.status_ptr(dev, "fused_linear_distillation"),
-                _lib.stream_ptr(dev),
+                1 if ids.dtype is torch.int64 else 0, ignore_index, logits.data_ptr(), _lib.dtype_code(logits.dtype),
+                n, v, k, top, temperature, loss.data_ptr(), list_ids, probs, z, stats, ws.data_ptr(), ws.numel(),
+                _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
             )
-        _lib.check(st, "fused_linear_distillation forward")
-        ctx.save_for_backward(h, w, list_ids, probs, z, stats)
-        ctx.temperature = temperature
-        ctx.dtypes = (hidden.dtype, weight.dtype)
+        if st:
+            _lib.check(st, op + " forward")
+        ctx.save_for_backward(h, w, kept)
+        ctx.args = (temperature, top, hidden.dtype, weight.dtype)
         return loss
 
     @staticmethod
@@ -62,29 +63,33 @@ class _FusedLinearDistillation(torch.autograd.Function):
         if not (need_h or need_w):
             return (None,) * 7
         lib = _lib.load()
-        h, w, list_ids, probs, z, stats = ctx.saved_tensors
+        op = "fused_linear_distillation"
+        h, w, kept = ctx.saved_tensors
+        temperature, top, h_dtype, w_dtype = ctx.args
         n, k = h.shape
-        v, top = w.shape[0], list_ids.shape[1]
+        v = w.shape[0]
         dev = h.device
-        dh = torch.empty((n, k), device=dev, dtype=ctx.dtypes[0]) if need_h else None
-        dw = torch.empty((v, k), device=dev, dtype=ctx.dtypes[1]) if need_w else None
-        go = grad_output.detach().to(device=dev, dtype=torch.float32).reshape(1).contiguous()
-        ws = torch.empty((int(lib.mt_distill_bwd_workspace_bytes(n, v, k)),), device=dev, dtype=torch.uint8)
+        dh = h.new_empty((n, k), dtype=h_dtype) if need_h else None
+        dw = w.new_empty((v, k), dtype=w_dtype) if need_w else None
+        go = grad_output if grad_output.dtype is torch.float32 else grad_output.float()
+        list_ids = kept.data_ptr()
+        probs, z, stats = (list_ids + 4 * n * top * i for i in (1, 2, 3))
+        ws = h.new_empty((lib.mt_distill_bwd_workspace_bytes(n, v, k),), dtype=torch.uint8)
         with _lib.on_device(dev):
             st = lib.mt_distill_bwd(
-                h.data_ptr(), w.data_ptr(), _lib.dtype_code(h.dtype), n, v, k, top, ctx.temperature,
-                list_ids.data_ptr(), probs.data_ptr(), z.data_ptr(), stats.data_ptr(), go.data_ptr(),
-                dh.data_ptr() if dh is not None else None, _lib.dtype_code(ctx.dtypes[0]),
-                dw.data_ptr() if dw is not None else None, _lib.dtype_code(ctx.dtypes[1]), ws.data_ptr(), ws.numel(),
-                _lib.status_ptr(dev, "fused_linear_distillation"), _lib.stream_ptr(dev),
+                h.data_ptr(), w.data_ptr(), _lib.dtype_code(h.dtype), n, v, k, top, temperature, list_ids, probs, z,
+                stats, go.data_ptr(), None if dh is None else dh.data_ptr(), _lib.dtype_code(h_dtype),
+                None if dw is None else dw.data_ptr(), _lib.dtype_code(w_dtype), ws.data_ptr(), ws.numel(),
+                _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
             )
-        _lib.check(st, "fused_linear_distillation backward")
+        if st:
+            _lib.check(st, op + " backward")
         return dh, dw, None, None, None, None, None
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and 16-byte aligned (a view at an odd offset is copied)."""
-    t = t.contiguous()
+def _aligned(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """``t`` in ``dtype``, contiguous and 16-byte aligned (a view at an odd offset is copied)."""
+    t = (t if t.dtype is dtype else t.to(dtype)).contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
