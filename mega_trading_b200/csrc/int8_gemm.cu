@@ -59,11 +59,16 @@ struct Int8Epilogue {
   }
 };
 
-// 8 lanes per channel, 4 channels per warp; MT tokens (rows past M repeat the last one).
+// 8 lanes per channel, 4 channels per warp, 32 channels per block; MT tokens
+// (rows past M are zero).  Blocks of 1,024 of K: a lane's 8 x 16 bytes of w are on
+// their way to registers before the tokens' part of x is staged, so all of w is
+// in flight at once (21,504 x 768: every block of the grid is resident).
 template <typename TO, int MT>
 __global__ void __launch_bounds__(256) int8_few_kernel(const int8_t* __restrict__ x, const float* __restrict__ xs,
                                                        const int8_t* __restrict__ w, const float* __restrict__ ws,
                                                        TO* __restrict__ y, int M, int N, int K) {
+  constexpr int kBlockK = 1024;
+  __shared__ __align__(16) int8_t sx[MT][kBlockK];
   const int sub = threadIdx.x & 7;
   const int n = (blockIdx.x * 256 + threadIdx.x) >> 3;
   const bool live = n < N;
@@ -71,16 +76,32 @@ __global__ void __launch_bounds__(256) int8_few_kernel(const int8_t* __restrict_
   int acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = 0;
-#pragma unroll 4
-  for (int k = sub * 16; k < K; k += 128) {
-    const int4 b = __ldg(reinterpret_cast<const int4*>(wr + k));
+  for (int k0 = 0; k0 < K; k0 += kBlockK) {
+    int4 b[8];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int4 a = __ldg(reinterpret_cast<const int4*>(x + int64_t(min(m, M - 1)) * K + k));
-      acc[m] = __dp4a(a.x, b.x, acc[m]);
-      acc[m] = __dp4a(a.y, b.y, acc[m]);
-      acc[m] = __dp4a(a.z, b.z, acc[m]);
-      acc[m] = __dp4a(a.w, b.w, acc[m]);
+    for (int i = 0; i < 8; ++i) {
+      const int k = k0 + i * 128 + sub * 16;
+      b[i] = k < K ? __ldg(reinterpret_cast<const int4*>(wr + k)) : make_int4(0, 0, 0, 0);
+    }
+    if (k0 > 0) __syncthreads();
+    for (int i = threadIdx.x; i < MT * (kBlockK / 16); i += 256) {
+      const int m = i / (kBlockK / 16), k = k0 + i % (kBlockK / 16) * 16;
+      *reinterpret_cast<int4*>(&sx[m][k - k0]) = m < M && k < K
+                                                     ? __ldg(reinterpret_cast<const int4*>(x + int64_t(m) * K + k))
+                                                     : make_int4(0, 0, 0, 0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (k0 + i * 128 >= K) break;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int4 a = *reinterpret_cast<const int4*>(&sx[m][i * 128 + sub * 16]);
+        acc[m] = __dp4a(a.x, b[i].x, acc[m]);
+        acc[m] = __dp4a(a.y, b[i].y, acc[m]);
+        acc[m] = __dp4a(a.z, b[i].z, acc[m]);
+        acc[m] = __dp4a(a.w, b[i].w, acc[m]);
+      }
     }
   }
 #pragma unroll

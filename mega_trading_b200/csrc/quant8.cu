@@ -55,8 +55,20 @@ __device__ __forceinline__ void store8f(T* p, const float (&v)[8]) {
   }
 }
 
-// max that keeps a NaN of either side out (fmaxf) but lets the caller see it
-// through the sum of squares or the products' own propagation.
+// max(a, |b|) that is NaN if either is.
+__device__ __forceinline__ float amax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+  return d;
+}
+
+// rint(v) for |v| <= 127 in the low byte: adding 1.5 * 2^23 leaves the integer,
+// rounded to even, in the low mantissa bits (FMA pipe instead of conversions).
+__device__ __forceinline__ uint32_t int8_bits(float v) { return __float_as_uint(__fadd_rn(v, 12582912.f)); }
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
 struct QParams {
   const void* x;
   const void* res;   // ADD
@@ -123,7 +135,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quant8_kernel(const __g
       }
     }
   }
-  float amax = 0.f, bad = 0.f;  // bad: NaN once any product is NaN (fmaxf drops NaNs)
+  float amax = 0.f;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     if constexpr (MODE != kPlain) {
@@ -155,14 +167,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quant8_kernel(const __g
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      amax = fmaxf(amax, fabsf(v[c][e]));
-      bad = fmaf(v[c][e], 0.f, bad);  // 0, or NaN from an infinity or a NaN
-    }
+    for (int e = 0; e < 8; ++e) amax = amax_nan(amax, v[c][e]);
   }
-  ss = ss + bad;  // a non-finite product makes the row's statistics NaN
-  ss = warp_sum(ss);
-  amax = warp_max(amax);
+  if constexpr (MODE != kPlain) ss = warp_sum(ss);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if constexpr (TPR > 32) {
     constexpr int kWarps = TPR / 32;
     const int base = (threadIdx.x / TPR) * kWarps;
@@ -176,38 +185,31 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quant8_kernel(const __g
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
       ss += red[0][base + i];
-      amax = fmaxf(amax, red[1][base + i]);
+      amax = amax_nan(amax, red[1][base + i]);
     }
   }
   if (!live) return;
-  const bool some = amax >= kTinyAmax;
-  const float inv = some ? __fdiv_rn(127.f, amax) : 0.f;
+  // an infinity or a NaN anywhere in the row: the scale is NaN
+  const bool finite = amax < INFINITY;
+  const float inv = finite && amax >= kTinyAmax ? __fdiv_rn(127.f, amax) : 0.f;
   if (t == 0) {
-    // plain rows: ss is 0, or NaN for a non-finite row
-    const float rs = MODE == kPlain ? 1.f + ss : rsqrtf(ss / float(dim) + p.eps);
-    p.scale[row] = some || isnan(ss) ? amax * rs / 127.f : 0.f;
+    const float rs = MODE == kPlain ? 1.f : rsqrtf(ss / float(dim) + p.eps);
+    p.scale[row] = !finite ? NAN : (amax >= kTinyAmax || isnan(rs) ? amax * rs / 127.f : 0.f);
   }
   int8_t* q = p.q + row * dim;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    int b[8];
+    uint32_t b[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) b[e] = __float2int_rn(__fmul_rn(v[c][e], inv));
+    for (int e = 0; e < 8; ++e) b[e] = int8_bits(__fmul_rn(v[c][e], inv));
     if constexpr (VEC) {
       const int col = col_of(c, 0);
-      if (col < dim) {
-        uint32_t lo = 0, hi = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          lo |= (uint32_t(b[e]) & 0xFFu) << (8 * e);
-          hi |= (uint32_t(b[e + 4]) & 0xFFu) << (8 * e);
-        }
-        *reinterpret_cast<uint2*>(q + col) = make_uint2(lo, hi);
-      }
+      if (col < dim)
+        *reinterpret_cast<uint2*>(q + col) = make_uint2(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (col_of(c, e) < dim) q[col_of(c, e)] = (int8_t)b[e];
+        if (col_of(c, e) < dim) q[col_of(c, e)] = (int8_t)(b[e] & 0xFFu);
     }
   }
 }
