@@ -84,6 +84,74 @@ struct QParams {
 
 enum { kPlain = 0, kNorm = 1, kAddNorm = 2 };
 
+// Two 16-bit maxima of magnitudes at a time, NaN if either is.
+template <typename T> struct Pair16;
+template <> struct Pair16<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct Pair16<__half> { using type = __half2; };
+template <typename T>
+__device__ __forceinline__ uint32_t amax2_nan(uint32_t a, uint32_t b) {
+  using P = typename Pair16<T>::type;
+  P r = __hmax2_nan(*reinterpret_cast<P*>(&a), __habs2(*reinterpret_cast<P*>(&b)));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// Plain rows of 16-bit values in 16-byte words: the maximum is exact in 16
+// bits, so the row is kept packed (half the registers of the general kernel,
+// more rows in flight) and widened once, when it is quantised.
+template <typename T, int TPR, int NC>
+__global__ void __launch_bounds__(256, 8) quant8_packed_kernel(const __grid_constant__ QParams p) {
+  static_assert(TPR <= 256, "one block's threads");
+  constexpr int kRows = 256 / TPR;
+  __shared__ float red[8];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / TPR;
+  const bool live = row < p.rows;
+  const T* x = static_cast<const T*>(p.x) + row * p.dim;
+  uint4 r[NC];
+  uint32_t m = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int col = (c * TPR + t) * 8;
+    r[c] = live && col < p.dim ? __ldg(reinterpret_cast<const uint4*>(x + col)) : make_uint4(0u, 0u, 0u, 0u);
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+    m = amax2_nan<T>(amax2_nan<T>(amax2_nan<T>(amax2_nan<T>(m, r[c].x), r[c].y), r[c].z), r[c].w);
+  float lo, hi;
+  unpack2<T>(m, lo, hi);
+  float amax = amax_nan(lo, hi);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if constexpr (TPR > 32) {
+    constexpr int kWarps = TPR / 32;
+    if (lane_id() == 0) red[warp_id()] = amax;
+    __syncthreads();
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) amax = amax_nan(amax, red[threadIdx.x / TPR * kWarps + i]);
+  }
+  if (!live) return;
+  const bool finite = amax < INFINITY;
+  const float inv = finite && amax >= kTinyAmax ? __fdiv_rn(127.f, amax) : 0.f;
+  if (t == 0) p.scale[row] = !finite ? NAN : (amax >= kTinyAmax ? amax / 127.f : 0.f);
+  int8_t* q = p.q + row * p.dim;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int col = (c * TPR + t) * 8;
+    const uint32_t w[4] = {r[c].x, r[c].y, r[c].z, r[c].w};
+    uint32_t b[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v0, v1;
+      unpack2<T>(w[e], v0, v1);
+      b[2 * e] = int8_bits(__fmul_rn(v0, inv));
+      b[2 * e + 1] = int8_bits(__fmul_rn(v1, inv));
+    }
+    if (col < p.dim)
+      *reinterpret_cast<uint2*>(q + col) = make_uint2(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]));
+  }
+}
+
 // TPR threads own a row; each holds NC chunks of 8 elements.
 template <typename TX, typename TR, int MODE, int TPR, int NC, bool VEC>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quant8_kernel(const __grid_constant__ QParams p) {
@@ -221,9 +289,12 @@ int launch_q(const QParams& p, bool vec, cudaStream_t s) {
   constexpr int kBlock = TPR < 256 ? 256 : TPR;
   const int64_t grid = (p.rows + kBlock / TPR - 1) / (kBlock / TPR);
   if (grid > 0x7fffffffLL) return MT_ERR_INVALID_ARGUMENT;
-  if (vec)
-    quant8_kernel<TX, TR, MODE, TPR, NC, true><<<(unsigned)grid, kBlock, 0, s>>>(p);
-  else
+  if (vec) {
+    if constexpr (MODE == kPlain && sizeof(TX) == 2 && TPR <= 256)
+      quant8_packed_kernel<TX, TPR, NC><<<(unsigned)grid, kBlock, 0, s>>>(p);
+    else
+      quant8_kernel<TX, TR, MODE, TPR, NC, true><<<(unsigned)grid, kBlock, 0, s>>>(p);
+  } else
     quant8_kernel<TX, TR, MODE, TPR, NC, false><<<(unsigned)grid, kBlock, 0, s>>>(p);
   return check_launch(MODE == kPlain ? "quantize_rows_int8" : "rms_norm_int8");
 }
