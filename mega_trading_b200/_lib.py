@@ -338,6 +338,13 @@ def require_one_device(op: str, first: torch.Tensor, *others: torch.Tensor) -> N
             raise RuntimeError(f"{op} requires all tensors on one device, found {first.device} and {t.device}")
 
 
+def refuse_second_derivative(op: str) -> None:
+    """For backward functions whose kernels build no graph: inside ``backward(create_graph=True)``
+    (the only time gradients are recorded there) raise instead of returning constants."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{op} has no second derivative; run the backward pass without create_graph")
+
+
 def launch_count() -> int:
     """Kernels the library has launched in this process (its own counter,
     ``mt_launch_count``); bench.py reports the difference over the timed region."""

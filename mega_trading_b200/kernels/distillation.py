@@ -14,7 +14,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -57,13 +56,13 @@ class _FusedLinearDistillation(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_output):
         need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         if not (need_h or need_w):
             return (None,) * 7
         lib = _lib.load()
         op = "fused_linear_distillation"
+        _lib.refuse_second_derivative(op)
         h, w, kept = ctx.saved_tensors
         temperature, top, h_dtype, w_dtype = ctx.args
         n, k = h.shape

@@ -12,7 +12,6 @@ atomics).
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -47,10 +46,9 @@ class _ScaledEmbedding(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_output):
-        if not ctx.needs_input_grad[0]:
-            return None, None, None, None, None
+        op = "scaled_embedding"
+        _lib.refuse_second_derivative(op)
         lib = _lib.load()
         (ids,) = ctx.saved_tensors
         scale, padding_idx, vocab, dim, wdtype = ctx.args
@@ -58,14 +56,16 @@ class _ScaledEmbedding(torch.autograd.Function):
         dev = g.device
         n = ids.numel()
         dw = g.new_empty((vocab, dim), dtype=wdtype)
-        ws = g.new_empty((lib.mt_embedding_bwd_workspace_bytes(n, vocab, dim),), dtype=torch.uint8)
+        ws_bytes = lib.mt_embedding_bwd_workspace_bytes(n, vocab, dim)
+        ws = g.new_empty((ws_bytes,), dtype=torch.uint8)
         with _lib.on_device(dev):
             st = lib.mt_embedding_bwd(
-                ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, n, g.data_ptr(), _lib.dtype_code(g.dtype),
-                vocab, dim, scale, padding_idx, dw.data_ptr(), _lib.dtype_code(wdtype), ws.data_ptr(), ws.numel(),
-                _lib.status_ptr(dev, "scaled_embedding"), _lib.stream_ptr(dev),
+                ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, n, g.data_ptr(), _lib.dtype_code(g.dtype),
+                vocab, dim, scale, padding_idx, dw.data_ptr(), _lib.dtype_code(wdtype), ws.data_ptr(), ws_bytes,
+                _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
             )
-        _lib.check(st, "scaled_embedding backward")
+        if st:
+            _lib.check(st, op + " backward")
         return dw, None, None, None, None
 
 

@@ -323,3 +323,14 @@ def test_distillation_in_a_graph_and_on_another_stream(cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_distillation_refuses_second_derivatives(cuda_device):
+    from mega_trading_b200.kernels.distillation import fused_linear_distillation
+
+    h = torch.randn(4, 16, device=cuda_device, dtype=BF16, requires_grad=True)
+    w = torch.randn(20, 16, device=cuda_device, dtype=BF16)
+    loss = fused_linear_distillation(h, w, torch.zeros(4, 1, dtype=torch.long, device=cuda_device),
+                                     torch.zeros(4, 1, device=cuda_device))
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(loss, h, create_graph=True)

@@ -211,3 +211,12 @@ def test_embedding_in_a_graph_and_on_another_stream(cuda_device):
     torch.cuda.synchronize()
     y3, d3 = step()
     assert torch.equal(y2, y3) and torch.equal(d2, d3) and not torch.equal(d2, d1)
+
+
+def test_embedding_refuses_second_derivatives(cuda_device):
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    w = torch.randn(10, 8, device=cuda_device, requires_grad=True)
+    y = scaled_embedding(torch.tensor([1, 2], device=cuda_device), w)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(y.sum(), w, create_graph=True)
