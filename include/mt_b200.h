@@ -405,7 +405,7 @@ MT_API int mt_distill_bwd(const void* hidden, const void* weight, int dtype, int
  * gradient.  Ids outside [0, vocab) give a zero output row, add to no gradient
  * and set the status word ((7 << 16) | 0xEEEE).
  * n, vocab < 2^31.  workspace: mt_embedding_bwd_workspace_bytes() bytes,
- * 256-byte aligned.
+ * 256-byte aligned (0 bytes for up to 256 ids: NULL will do).
  * ------------------------------------------------------------------- */
 MT_API int mt_embedding_fwd(const void* ids, int ids_i64, int64_t n, const void* weight,
                             int w_dtype, int64_t vocab, int64_t dim, float scale, void* out,

@@ -25,7 +25,8 @@
 // A run that lies inside its range goes straight to dW; a run cut by a border
 // leaves fp32 partial sums, at most two per range, which embed_join_kernel adds
 // up (it also zeroes the rows no token chose).  Every sum has a fixed order (no
-// atomics on values): results are the same each time.
+// atomics on values): results are the same each time.  Up to 256 tokens take one
+// launch that looks each row's tokens up instead (no sort, no workspace).
 //
 // Ids outside [0, V) read nothing: their output row is zero, they add to no
 // gradient and the status word is set.  Places holding padding_idx look up
@@ -754,6 +755,67 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const uint2* __restrict
 }
 
 // ---------------------------------------------------------------------------
+// a few tokens: one launch, no workspace
+// ---------------------------------------------------------------------------
+// A block writes 32 rows of dW and a warp four of them: it looks its ids up in
+// the token list (in shared memory) and adds the rows of dy that name them, in
+// the order of their positions, eight at a time.  For up to kFew tokens the
+// whole list is 256 compares per row and the longest sum 32 steps.
+constexpr int kFew = 256;
+
+template <typename TG, typename TD, bool VEC>
+__global__ void __launch_bounds__(256) embed_few_kernel(SortIn in, int n_tokens, const TG* __restrict__ dy, int dim,
+                                                        float scale, TD* __restrict__ dw) {
+  constexpr int E = lane_elems<TG, TD>();
+  using C = Cols<E, VEC>;
+  __shared__ uint32_t keys[kFew];
+  __shared__ uint16_t found[8][kFew];
+  const int lane = lane_id(), w = warp_id();
+  {
+    const int i = threadIdx.x;
+    const int64_t id = i < n_tokens ? load_id(in.ids, in.i64, i) : 0;
+    keys[i] = i < n_tokens ? key_of(in, id) : 0xffffffffu;
+    if (blockIdx.x == 0 && i < n_tokens) report_id(in, id);
+  }
+  __syncthreads();
+  for (int r = 0; r < 4; ++r) {
+    const int64_t v = int64_t(blockIdx.x) * 32 + w * 4 + r;
+    if (v >= in.vocab) break;
+    int count = 0;
+    for (int i0 = 0; i0 < n_tokens; i0 += 32) {
+      const uint32_t hits = __ballot_sync(0xffffffffu, keys[i0 + lane] == (uint32_t)v);
+      if (hits >> lane & 1u) found[w][count + __popc(hits & ((1u << lane) - 1u))] = (uint16_t)(i0 + lane);
+      count += __popc(hits);
+    }
+    __syncwarp();
+    for (int c0 = 0; c0 < dim; c0 += C::kSlab) {
+      float acc[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+      for (int q = 0; q < count; q += 8) {
+        float x[8][E];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (q + j < count) {
+            C::load(dy + int64_t(found[w][q + j]) * dim, c0, dim, x[j]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[j][e] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          acc[e] += ((x[0][e] + x[1][e]) + (x[2][e] + x[3][e])) + ((x[4][e] + x[5][e]) + (x[6][e] + x[7][e]));
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= scale;
+      C::store(dw + v * dim, c0, dim, acc);
+    }
+    __syncwarp();
+  }
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -841,7 +903,7 @@ extern "C" int mt_embedding_fwd(const void* ids, int ids_i64, int64_t n, const v
 }
 
 extern "C" int64_t mt_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t dim) {
-  if (n <= 0 || check_embed(n, vocab, dim) != MT_OK) return 256;
+  if (n <= kFew || check_embed(n, vocab, dim) != MT_OK) return 0;
   return plan_embed(n, vocab, dim).bytes;
 }
 
@@ -864,6 +926,21 @@ extern "C" int mt_embedding_bwd(const void* ids, int ids_i64, int64_t n, const v
     return MT_OK;
   }
   if (ids == nullptr || dout == nullptr || status == nullptr) return MT_ERR_INVALID_ARGUMENT;
+  if (n <= kFew) {
+    if ((st = bind_device_of(dweight)) != MT_OK) return st;
+    const SortIn few{ids, ids_i64, vocab, padding_idx < 0 ? int64_t(-1) : padding_idx, status};
+    return with_type(dout_dtype, [&](auto gv) {
+      return with_type(dw_dtype, [&](auto dv) {
+        using TG = decltype(gv);
+        using TD = decltype(dv);
+        const bool vec = on16(dout) && on16(dweight) && dim % lane_elems<TG, TD>() == 0;
+        auto kern = vec ? embed_few_kernel<TG, TD, true> : embed_few_kernel<TG, TD, false>;
+        kern<<<(unsigned)((vocab + 31) / 32), 256, 0, s>>>(few, (int)n, static_cast<const TG*>(dout), (int)dim, scale,
+                                                           static_cast<TD*>(dweight));
+        return check_launch("embedding_bwd_few");
+      });
+    });
+  }
   const EmbedPlan pl = plan_embed(n, vocab, dim);
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || workspace_bytes < pl.bytes)
     return MT_ERR_WORKSPACE;

@@ -47,26 +47,51 @@ class _ScaledEmbedding(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
-        op = "scaled_embedding"
-        _lib.refuse_second_derivative(op)
-        lib = _lib.load()
         (ids,) = ctx.saved_tensors
-        scale, padding_idx, vocab, dim, wdtype = ctx.args
-        g = grad_output.contiguous()
-        dev = g.device
-        n = ids.numel()
-        dw = g.new_empty((vocab, dim), dtype=wdtype)
-        ws_bytes = lib.mt_embedding_bwd_workspace_bytes(n, vocab, dim)
-        ws = g.new_empty((ws_bytes,), dtype=torch.uint8)
-        with _lib.on_device(dev):
-            st = lib.mt_embedding_bwd(
-                ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, n, g.data_ptr(), _lib.dtype_code(g.dtype),
-                vocab, dim, scale, padding_idx, dw.data_ptr(), _lib.dtype_code(wdtype), ws.data_ptr(), ws_bytes,
-                _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
-            )
-        if st:
-            _lib.check(st, op + " backward")
-        return dw, None, None, None, None
+        if torch.is_grad_enabled() and grad_output.requires_grad:
+            return _EmbeddingGradient.apply(grad_output, ids, ctx.args), None, None, None, None
+        return _gradient(grad_output, ids, *ctx.args), None, None, None, None
+
+
+def _gradient(grad_output, ids, scale, padding_idx, vocab, dim, dtype):
+    """The table's dense gradient in ``dtype``."""
+    op = "scaled_embedding"
+    lib = _lib.load()
+    g = grad_output.contiguous()
+    dev = g.device
+    n = ids.numel()
+    dw = g.new_empty((vocab, dim), dtype=dtype)
+    ws_bytes = lib.mt_embedding_bwd_workspace_bytes(n, vocab, dim)
+    ws = g.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    with _lib.on_device(dev):
+        st = lib.mt_embedding_bwd(
+            ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, n, g.data_ptr(), _lib.dtype_code(g.dtype), vocab,
+            dim, scale, padding_idx, dw.data_ptr(), _lib.dtype_code(dtype), ws.data_ptr() if ws_bytes else None,
+            ws_bytes, _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
+        )
+    if st:
+        _lib.check(st, op + " backward")
+    return dw
+
+
+class _EmbeddingGradient(torch.autograd.Function):
+    """The gradient as a (linear) function of the output's gradient, for ``create_graph=True``:
+    its own gradient is the lookup again, with the padded places left out."""
+
+    @staticmethod
+    def forward(ctx, grad_output, ids, args):
+        ctx.save_for_backward(ids)
+        ctx.args, ctx.dtype = args, grad_output.dtype
+        return _gradient(grad_output, ids, *args)
+
+    @staticmethod
+    def backward(ctx, grad_table):
+        (ids,) = ctx.saved_tensors
+        scale, padding_idx = ctx.args[:2]
+        out = scaled_embedding(ids, grad_table, scale=scale, out_dtype=ctx.dtype)
+        if padding_idx >= 0:
+            out = out * (ids != padding_idx).unsqueeze(-1)
+        return out, None, None
 
 
 def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: int | None = None,

@@ -103,9 +103,12 @@ class RMSNorm(nn.Module):
 
 
 class TokenEmbedding(nn.Embedding):
-    """The token table; lookup and sorted-token gradient by ``kernels.embedding``."""
+    """The token table; lookup and sorted-token gradient by ``kernels.embedding`` (torch's own
+    lookup while the table is on the host)."""
 
     def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
+        if not self.weight.is_cuda:
+            return super().forward(input_ids)
         return scaled_embedding(input_ids, self.weight, padding_idx=self.padding_idx)
 
 

@@ -49,6 +49,10 @@ def _check_grad(dw, ids, grad, vocab, scale, pad):
 @pytest.mark.parametrize("n,vocab,dim,kind,wt,ot,scale,pad,seed", [
     (1, 21504, 768, "uniform", F32, F32, 1.0, None, 1),
     (16, 21504, 768, "uniform", F32, BF16, 27.7, None, 2),
+    (256, 21504, 768, "same", F32, F32, 2.0, None, 18),       # the most tokens that take one launch
+    (200, 30, 509, "skewed", BF16, F32, 1.0, 4, 19),
+    (255, 1001, 1032, "skewed", F16, F16, 1.0, 1000, 20),
+    (257, 21504, 64, "uniform", F32, F32, 1.0, None, 21),
     (4096, 21504, 256, "skewed", F32, F32, 1.0, None, 3),     # the largest single-block sort
     (4097, 21504, 256, "skewed", F32, F32, 1.0, None, 4),     # the smallest tiled sort
     (20000, 21504, 768, "skewed", F32, F32, 1.0, 0, 5),
@@ -213,10 +217,36 @@ def test_embedding_in_a_graph_and_on_another_stream(cuda_device):
     assert torch.equal(y2, y3) and torch.equal(d2, d3) and not torch.equal(d2, d1)
 
 
-def test_embedding_refuses_second_derivatives(cuda_device):
+def test_embedding_second_derivative(cuda_device):
+    """The gradient is linear in the output's gradient; differentiating it gives the lookup back."""
     from mega_trading_b200.kernels.embedding import scaled_embedding
 
-    w = torch.randn(10, 8, device=cuda_device, requires_grad=True)
-    y = scaled_embedding(torch.tensor([1, 2], device=cuda_device), w)
-    with pytest.raises(RuntimeError, match="no second derivative"):
-        torch.autograd.grad(y.sum(), w, create_graph=True)
+    gen = torch.Generator(device=cuda_device).manual_seed(1)
+    ids = torch.tensor([1, 2, 1, 5, 9], device=cuda_device)
+    w = torch.randn(10, 8, device=cuda_device, generator=gen, requires_grad=True)
+    g = torch.randn(5, 8, device=cuda_device, generator=gen, requires_grad=True)
+    u = torch.randn(10, 8, device=cuda_device, generator=gen, requires_grad=True)
+    y = scaled_embedding(ids, w, scale=2.0, padding_idx=9)
+    (dw,) = torch.autograd.grad(y, w, g, create_graph=True)
+    dg, du = torch.autograd.grad((dw * u).sum(), (g, u), create_graph=True)
+    want = 2.0 * u.detach()[ids]
+    want[4] = 0
+    assert torch.equal(dg.detach(), want) and torch.equal(du.detach(), dw.detach())
+    (again,) = torch.autograd.grad((dg * g.detach()).sum(), u)
+    assert torch.equal(again, dw.detach())
+    # create_graph without a differentiable gradient is the plain gradient
+    (plain,) = torch.autograd.grad(scaled_embedding(ids, w, scale=2.0, padding_idx=9), w, g.detach(), create_graph=True)
+    assert torch.equal(plain, dw.detach())
+
+
+@pytest.mark.parametrize("n", [90, 700])
+def test_embedding_gradient_off_the_vector_grid(cuda_device, n):
+    """A contiguous output gradient whose base is not 16-byte aligned."""
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    gen = torch.Generator(device=cuda_device).manual_seed(n)
+    ids = torch.randint(0, 60, (n,), device=cuda_device, generator=gen)
+    w = torch.randn(60, 64, device=cuda_device, generator=gen, requires_grad=True)
+    g = torch.randn(n * 64 + 1, device=cuda_device, generator=gen)[1:].view(n, 64)
+    (dw,) = torch.autograd.grad(scaled_embedding(ids, w), w, g)
+    _check_grad(dw, ids, g, 60, 1.0, None)

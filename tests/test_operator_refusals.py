@@ -138,3 +138,12 @@ def test_distillation_refusals():
         fused_linear_distillation(h[:, :4], w[:, :4], ids, lg)
     with pytest.raises(ValueError, match="compute_weight"):
         fused_linear_distillation(h, w, ids, lg, compute_weight=w[:3])
+
+
+def test_token_table_on_the_host_still_looks_up():
+    from mega_trading_b200.model import ModelConfig, TradingModelB200
+
+    m = TradingModelB200(ModelConfig(vocab_size=50, block_size=16, hidden_dim=32, layers=1, attention_heads=4,
+                                     kv_heads=2, intermediate_dim=48))
+    ids = torch.tensor([[1, 2, 3]])
+    assert torch.equal(m.token_embedding(ids), m.token_embedding.weight[ids])
