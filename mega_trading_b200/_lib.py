@@ -184,29 +184,18 @@ def stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
 
 
-class _Here:
-    """Context of a call whose device is already current."""
-
-    def __enter__(self) -> None:
-        pass
-
-    def __exit__(self, *exc) -> None:
-        pass
-
-
-_HERE = _Here()
-
-
-def on_device(device: torch.device):
-    """Context that makes ``device`` current for a launch (nothing to do when it already is)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
-
-
 def i64_array(values) -> ctypes.Array:
     arr = (ctypes.c_int64 * len(values))(*[int(v) for v in values])
     return arr
+
+
+def call(fn, device: torch.device, *args) -> int:
+    """``fn(*args)`` with ``device`` current (launches go to the current device's context)."""
+    idx = device.index
+    if idx is None or idx == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(idx):
+        return fn(*args)
 
 
 # Per-device uint32 status word for the bounded device waits.
@@ -331,8 +320,9 @@ def require_cuda_sm100(t: torch.Tensor, op: str) -> None:
 
 def require_one_device(op: str, first: torch.Tensor, *others: torch.Tensor) -> None:
     """All tensors on one sm_100 device."""
-    require_cuda_sm100(first, op)
-    idx = first.get_device()
+    idx = first.get_device()  # -1 on the host
+    if idx not in _sm100:
+        require_cuda_sm100(first, op)
     for t in others:
         if t.get_device() != idx:
             raise RuntimeError(f"{op} requires all tensors on one device, found {first.device} and {t.device}")

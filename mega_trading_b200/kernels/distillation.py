@@ -42,13 +42,12 @@ class _FusedLinearDistillation(torch.autograd.Function):
         list_ids = kept.data_ptr()
         probs, z, stats = (list_ids + 4 * n * top * i for i in (1, 2, 3))
         ws = h.new_empty((lib.mt_distill_workspace_bytes(n, v),), dtype=torch.uint8)
-        with _lib.on_device(dev):
-            st = lib.mt_distill_fwd(
-                h.data_ptr(), w.data_ptr(), _lib.dtype_code(cdtype), ids.data_ptr(),
-                1 if ids.dtype is torch.int64 else 0, ignore_index, logits.data_ptr(), _lib.dtype_code(logits.dtype),
-                n, v, k, top, temperature, loss.data_ptr(), list_ids, probs, z, stats, ws.data_ptr(), ws.numel(),
-                _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
-            )
+        st = _lib.call(
+            lib.mt_distill_fwd, dev, h.data_ptr(), w.data_ptr(), _lib.dtype_code(cdtype), ids.data_ptr(),
+            1 if ids.dtype is torch.int64 else 0, ignore_index, logits.data_ptr(), _lib.dtype_code(logits.dtype), n, v,
+            k, top, temperature, loss.data_ptr(), list_ids, probs, z, stats, ws.data_ptr(), ws.numel(),
+            _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
+        )
         if st:
             _lib.check(st, op + " forward")
         ctx.save_for_backward(h, w, kept)
@@ -74,13 +73,12 @@ class _FusedLinearDistillation(torch.autograd.Function):
         list_ids = kept.data_ptr()
         probs, z, stats = (list_ids + 4 * n * top * i for i in (1, 2, 3))
         ws = h.new_empty((lib.mt_distill_bwd_workspace_bytes(n, v, k),), dtype=torch.uint8)
-        with _lib.on_device(dev):
-            st = lib.mt_distill_bwd(
-                h.data_ptr(), w.data_ptr(), _lib.dtype_code(h.dtype), n, v, k, top, temperature, list_ids, probs, z,
-                stats, go.data_ptr(), None if dh is None else dh.data_ptr(), _lib.dtype_code(h_dtype),
-                None if dw is None else dw.data_ptr(), _lib.dtype_code(w_dtype), ws.data_ptr(), ws.numel(),
-                _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
-            )
+        st = _lib.call(
+            lib.mt_distill_bwd, dev, h.data_ptr(), w.data_ptr(), _lib.dtype_code(h.dtype), n, v, k, top, temperature,
+            list_ids, probs, z, stats, go.data_ptr(), None if dh is None else dh.data_ptr(), _lib.dtype_code(h_dtype),
+            None if dw is None else dw.data_ptr(), _lib.dtype_code(w_dtype), ws.data_ptr(), ws.numel(),
+            _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
+        )
         if st:
             _lib.check(st, op + " backward")
         return dh, dw, None, None, None, None, None

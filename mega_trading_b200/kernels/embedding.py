@@ -26,12 +26,11 @@ def _lookup(weight, ids, scale, out_dtype):
     vocab, dim = w.shape
     dev = w.device
     out = w.new_empty((*ids.shape, dim), dtype=out_dtype)
-    with _lib.on_device(dev):
-        st = _lib.load().mt_embedding_fwd(
-            ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, ids.numel(), w.data_ptr(), _lib.dtype_code(w.dtype),
-            vocab, dim, scale, out.data_ptr(), _lib.dtype_code(out_dtype), _lib.status_ptr(dev, "scaled_embedding"),
-            _lib.stream_ptr(dev),
-        )
+    st = _lib.call(
+        _lib.load().mt_embedding_fwd, dev, ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, ids.numel(),
+        w.data_ptr(), _lib.dtype_code(w.dtype), vocab, dim, scale, out.data_ptr(), _lib.dtype_code(out_dtype),
+        _lib.status_ptr(dev, "scaled_embedding"), _lib.stream_ptr(dev),
+    )
     if st:
         _lib.check(st, "scaled_embedding forward")
     return ids, out
@@ -63,12 +62,11 @@ def _gradient(grad_output, ids, scale, padding_idx, vocab, dim, dtype):
     dw = g.new_empty((vocab, dim), dtype=dtype)
     ws_bytes = lib.mt_embedding_bwd_workspace_bytes(n, vocab, dim)
     ws = g.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-    with _lib.on_device(dev):
-        st = lib.mt_embedding_bwd(
-            ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, n, g.data_ptr(), _lib.dtype_code(g.dtype), vocab,
-            dim, scale, padding_idx, dw.data_ptr(), _lib.dtype_code(dtype), ws.data_ptr() if ws_bytes else None,
-            ws_bytes, _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
-        )
+    st = _lib.call(
+        lib.mt_embedding_bwd, dev, ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, n, g.data_ptr(),
+        _lib.dtype_code(g.dtype), vocab, dim, scale, padding_idx, dw.data_ptr(), _lib.dtype_code(dtype),
+        ws.data_ptr() if ws_bytes else None, ws_bytes, _lib.status_ptr(dev, op), _lib.stream_ptr(dev),
+    )
     if st:
         _lib.check(st, op + " backward")
     return dw

@@ -69,13 +69,11 @@ def _norm(op: str, hidden, residual, weight, eps: float):
         r = residual.contiguous()
         new = torch.empty_like(r)
         rcode, r_ptr, new_ptr = _lib.dtype_code(r.dtype), r.data_ptr(), new.data_ptr()
-    q = x.new_empty(x.shape, dtype=torch.int8)
+    q = torch.empty_like(x, dtype=torch.int8)
     scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     dev = x.device
-    with _lib.on_device(dev):
-        st = _lib.load().mt_rms_norm_int8(x.data_ptr(), code, r_ptr, rcode, w.data_ptr(), _lib.dtype_code(wdt),
-                                          new_ptr, q.data_ptr(), scale.data_ptr(), rows, dim, eps,
-                                          _lib.stream_ptr(dev))
+    st = _lib.call(_lib.load().mt_rms_norm_int8, dev, x.data_ptr(), code, r_ptr, rcode, w.data_ptr(),
+                   _lib.dtype_code(wdt), new_ptr, q.data_ptr(), scale.data_ptr(), rows, dim, eps, _lib.stream_ptr(dev))
     if st:
         _lib.check(st, op)
     return new, q, scale
@@ -109,12 +107,11 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     _check(op, x)
     rows, dim = _rows(op, x)
     xc = x.contiguous()
-    q = xc.new_empty(xc.shape, dtype=torch.int8)
+    q = torch.empty_like(xc, dtype=torch.int8)
     scale = xc.new_empty(xc.shape[:-1], dtype=torch.float32)
     dev = x.device
-    with _lib.on_device(dev):
-        st = _lib.load().mt_quantize_rows_int8(xc.data_ptr(), _lib.dtype_code(x.dtype), q.data_ptr(),
-                                               scale.data_ptr(), rows, dim, _lib.stream_ptr(dev))
+    st = _lib.call(_lib.load().mt_quantize_rows_int8, dev, xc.data_ptr(), _lib.dtype_code(x.dtype), q.data_ptr(),
+                   scale.data_ptr(), rows, dim, _lib.stream_ptr(dev))
     if st:
         _lib.check(st, op)
     return q, scale
@@ -149,10 +146,9 @@ def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     xc, w, ws = _aligned(x), _aligned(weight), _aligned(weight_scale)
     xs = x_scale.contiguous()
     dev = x.device
-    with _lib.on_device(dev):
-        st = _lib.load().mt_int8_gemm(xc.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(),
-                                      _lib.dtype_code(out_dtype), x.numel() // k, n, k, _lib.status_ptr(dev, op),
-                                      _lib.stream_ptr(dev))
+    st = _lib.call(_lib.load().mt_int8_gemm, dev, xc.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(),
+                   y.data_ptr(), _lib.dtype_code(out_dtype), x.numel() // k, n, k, _lib.status_ptr(dev, op),
+                   _lib.stream_ptr(dev))
     if st:
         _lib.check(st, op)
     return y
