@@ -29,6 +29,12 @@
 // fp16 values are held times 2^15 for the same reason (|q - p| <= 1).  The rounding of
 // dz to 16 bits (half a step of its own magnitude) is the tensor cores' operand
 // type and the one rounding between the fp32 logits and the fp32 sums.
+//
+// Bound by the tensor pipe and, in a steady stream, by the power limit: 32,768
+// rows x 768 against 21,504 entries, forward and backward, 3.86 ms (8 NVK
+// operations at 1.13 PFLOP/s).  Alone: statistics 759 us (tensor pipe 81 %
+// busy), per 6,144-row chunk dz 148 us (82 %), dh 130 us (93 %), dW 144 us (81 %:
+// 252 tiles on 74 CTA pairs).
 #include <cmath>
 
 #include "tile_gemm.cuh"

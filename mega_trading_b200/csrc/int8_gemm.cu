@@ -5,7 +5,8 @@
 // the output type.  No counterpart in the reference (bf16 projections).
 //
 // Many tokens: the tcgen05 product of tile_gemm.cuh with kind::i8 (twice the
-// rate of 16-bit operands), scales in the epilogue.  Few tokens (M <= 16): the
+// rate of 16-bit operands), scales in the epilogue: 65,537 x 5,632 x 1,024 to
+// bf16 in 0.37 ms (2.0 POP/s; at K = 8,192 2.95 POP/s).  Few tokens (M <= 16): the
 // product is bound by reading w once and by latency, and a 128-row MMA tile
 // would be almost empty, so a dot-product kernel reads w straight into
 // registers (16 bytes per lane, 8 lanes per channel) and multiplies with dp4a.
