@@ -6,7 +6,7 @@
 //
 // Many tokens: the tcgen05 product of tile_gemm.cuh with kind::i8 (twice the
 // rate of 16-bit operands), scales in the epilogue: 65,537 x 5,632 x 1,024 to
-// bf16 in 0.37 ms (2.0 POP/s; at K = 8,192 2.95 POP/s).  Few tokens (M <= 16): the
+// bf16 in 0.37 ms (2.0 POP/s; at K = 8,192 2.95 POP/s).  Few tokens (M <= 8): the
 // product is bound by reading w once and by latency, and a 128-row MMA tile
 // would be almost empty, so a dot-product kernel reads w straight into
 // registers (16 bytes per lane, 8 lanes per channel) and multiplies with dp4a.
@@ -17,7 +17,9 @@ namespace {
 
 constexpr uint32_t kKernelId = 9;
 constexpr int kMaxK = 131056;
-constexpr int kFewTokens = 16;
+// us, dot products / 128 x 128 tiles: 21,504 x 768 with 4 tokens 5.1 / 8.2, 8
+// tokens 8.0 / 8.9, 16 tokens 13.8 / 8.8; 1,280 x 768 2.3 / 4.9, 3.2 / 4.8, 4.5 / 4.8
+constexpr int kFewTokens = 8;
 
 template <typename TO>
 struct Int8Epilogue {
@@ -126,10 +128,8 @@ int launch_few(const int8_t* x, const float* xs, const int8_t* w, const float* w
     int8_few_kernel<TO, 2><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
   else if (M <= 4)
     int8_few_kernel<TO, 4><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
-  else if (M <= 8)
-    int8_few_kernel<TO, 8><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
   else
-    int8_few_kernel<TO, 16><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
+    int8_few_kernel<TO, 8><<<grid, 256, 0, s>>>(x, xs, w, ws, y, M, N, K);
   return check_launch("int8_gemm_few");
 }
 
@@ -163,10 +163,12 @@ int run_int8(const int8_t* x, const float* xs, const int8_t* w, const float* ws,
              int N, int K, uint32_t* status, cudaStream_t s) {
   TO* y = static_cast<TO*>(out);
   if (M <= kFewTokens) return launch_few<TO>(x, xs, w, ws, y, M, N, K, s);
-  // CTA pairs need enough 256 x 256 tiles to occupy most of the GPU; smaller
-  // products take 128 x 128 tiles, four times as many.
+  // CTA pairs from one and a half 256 x 256 tiles per pair on; smaller products
+  // take 128 x 128 tiles, four times as many.  us, pairs / single, by tiles of
+  // a pair: 80 (4,096 x 1,280 x 768) 12.4 / 10.1, 64 (1,024 x 4,096 x 1,024) 10.3 / 9.2,
+  // 128 (2,048 x 4,096 x 1,024) 13.8 / 14.8, 336 (1,024 x 21,504 x 768) 22.6 / 25.4
   const int64_t pair_tiles = int64_t((M + 255) / 256) * ((N + 255) / 256);
-  if (pair_tiles >= get_sm_count() / 2)
+  if (4 * pair_tiles >= 3 * get_sm_count())
     return launch_tiles<TileCfg<kKindI8, false, false, 256, true, 16>, TO>(x, xs, w, ws, y, out_dtype, M, N, K, status, s);
   return launch_tiles<TileCfg<kKindI8, false, false, 128, false, 16>, TO>(x, xs, w, ws, y, out_dtype, M, N, K, status, s);
 }

@@ -53,8 +53,10 @@ def _check_grad(dw, ids, grad, vocab, scale, pad):
     (200, 30, 509, "skewed", BF16, F32, 1.0, 4, 19),
     (255, 1001, 1032, "skewed", F16, F16, 1.0, 1000, 20),
     (257, 21504, 64, "uniform", F32, F32, 1.0, None, 21),
-    (4096, 21504, 256, "skewed", F32, F32, 1.0, None, 3),     # the largest single-block sort
-    (4097, 21504, 256, "skewed", F32, F32, 1.0, None, 4),     # the smallest tiled sort
+    (2048, 21504, 256, "skewed", F32, F32, 1.0, None, 22),    # the largest single-block sort
+    (2049, 21504, 256, "skewed", F32, F32, 1.0, None, 23),    # the smallest tiled sort
+    (4096, 21504, 256, "skewed", F32, F32, 1.0, None, 3),
+    (4097, 21504, 256, "skewed", F32, F32, 1.0, None, 4),
     (20000, 21504, 768, "skewed", F32, F32, 1.0, 0, 5),
     (30011, 1000, 1000, "uniform", BF16, BF16, 31.6, 999, 6),
     (5000, 300, 509, "uniform", F16, F16, 0.5, None, 7),      # odd width: single-element accesses

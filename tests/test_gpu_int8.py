@@ -56,6 +56,9 @@ def _close(a, b, rtol):
     (130, 1023, torch.float16, torch.float16, torch.float32, 10),
     (4, 9001, torch.bfloat16, torch.bfloat16, torch.float32, 11),
     (1, 8, torch.bfloat16, torch.float32, torch.float32, 12),
+    (700, 768, torch.bfloat16, torch.float32, torch.float32, 13),   # enough rows for one warp each
+    (601, 1001, torch.float16, torch.float32, torch.float32, 14),
+    (3, 4096, torch.bfloat16, torch.float32, torch.float32, 15),
 ])
 def test_norm_int8_matches_definition(cuda_device, rows, dim, act, res, wdt, seed):
     from mega_trading_b200.kernels import int8
@@ -200,14 +203,17 @@ def _product(dev, m, k, n, out, seed, extreme=False):
     (3, 1024, 1280, torch.float16, 3),
     (8, 2816, 1024, torch.bfloat16, 4),
     (16, 400, 333, torch.float32, 5),
-    (17, 768, 768, torch.bfloat16, 6),        # first tensor-core size
+    (9, 768, 768, torch.bfloat16, 16),        # first tensor-core size
+    (17, 768, 768, torch.bfloat16, 6),
     (100, 16, 64, torch.float32, 7),          # one K stage, mostly zero fill
     (129, 144, 130, torch.bfloat16, 8),       # ragged in every dimension, rows off the 16-byte grid
     (200, 4112, 257, torch.float16, 9),
     (300, 768, 7, torch.float32, 10),
-    (1000, 1024, 4096, torch.bfloat16, 11),   # CTA pairs, ragged rows
+    (1000, 1024, 4096, torch.bfloat16, 11),   # below the pairs' size
+    (2000, 1024, 4096, torch.bfloat16, 14),   # CTA pairs, ragged rows
     (4097, 256, 2310, torch.float32, 12),     # CTA pairs, fp32, ragged columns
-    (5000, 2816, 1023, torch.float16, 13),    # CTA pairs, plain stores
+    (5000, 2816, 1023, torch.float16, 13),    # plain stores
+    (8000, 272, 1023, torch.bfloat16, 15),    # CTA pairs, plain stores
 ])
 def test_int8_linear_matches_definition(cuda_device, m, k, n, out, seed):
     _product(cuda_device, m, k, n, out, seed)
