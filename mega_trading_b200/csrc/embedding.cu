@@ -42,8 +42,11 @@ namespace mt {
 namespace {
 
 constexpr uint32_t kKernelId = 7;
-constexpr int kRounds = 4;       // 32-token rounds a warp ranks at a time
-constexpr int kSubTile = 8 * 32 * kRounds;  // tokens one sort block ranks at a time
+constexpr int kRounds = 4;  // 32-token rounds a warp ranks at a time
+// Warps of a sort block: 16 halve the tiles whose histograms every block sums
+// (whole gradient of 262,144 tokens x 768: 169 us, 8 warps 178), 8 start sooner
+// (5,000 tokens: 35.8 us, 16 warps 40.4).
+int sort_warps(int64_t n) { return n >= 65536 ? 16 : 8; }
 constexpr int kOneRounds = 2;
 constexpr int kOneBlock = 1024 * kOneRounds;  // tokens the single-block sort takes (whole gradient of 1,000
                                               // tokens x 768: 34.7 us, tiled 38.9; of 4,096: 41.6 / 36.5)
@@ -322,11 +325,13 @@ __global__ void __launch_bounds__(1024) embed_sort_small_kernel(SortIn in, int n
 
 // Histogram of the first digit per tile; clears the later passes' histograms
 // and the id ranges.
-__global__ void __launch_bounds__(256) embed_hist_kernel(SortIn in, int64_t n_tokens, int64_t tile,
+template <int NW>
+__global__ void __launch_bounds__(NW * 32) embed_hist_kernel(SortIn in, int64_t n_tokens, int64_t tile,
                                                          uint32_t* __restrict__ hist, int64_t hist_words, uint2* seg) {
+  constexpr int kSortThreads = NW * 32, kSubTile = kSortThreads * kRounds;
   __shared__ uint32_t h[256];
-  h[threadIdx.x] = 0;
-  const int64_t gid = int64_t(blockIdx.x) * 256 + threadIdx.x, gsz = int64_t(gridDim.x) * 256;
+  if (threadIdx.x < 256) h[threadIdx.x] = 0;
+  const int64_t gid = int64_t(blockIdx.x) * kSortThreads + threadIdx.x, gsz = int64_t(gridDim.x) * kSortThreads;
   const int64_t own = int64_t(gridDim.x) * 256;  // this pass's histograms
   for (int64_t i = own + gid; i < hist_words; i += gsz) hist[i] = 0;
   for (int64_t v = gid; v <= in.vocab; v += gsz) seg[v] = make_uint2(0u, 0u);
@@ -336,12 +341,12 @@ __global__ void __launch_bounds__(256) embed_hist_kernel(SortIn in, int64_t n_to
     int64_t id[kRounds];
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
-      const int64_t n = s0 + i * 256 + threadIdx.x;
+      const int64_t n = s0 + i * kSortThreads + threadIdx.x;
       id[i] = n < hi ? load_id(in.ids, in.i64, n) : -1;
     }
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
-      const bool live = s0 + i * 256 + threadIdx.x < hi;
+      const bool live = s0 + i * kSortThreads + threadIdx.x < hi;
       const uint32_t d = live ? key_of(in, id[i]) & 255u : 256u;
       if (live) report_id(in, id[i]);
       const uint32_t peers = __match_any_sync(0xffffffffu, d);
@@ -349,18 +354,19 @@ __global__ void __launch_bounds__(256) embed_hist_kernel(SortIn in, int64_t n_to
     }
   }
   __syncthreads();
-  hist[int64_t(blockIdx.x) * 256 + threadIdx.x] = h[threadIdx.x];
+  if (threadIdx.x < 256) hist[int64_t(blockIdx.x) * 256 + threadIdx.x] = h[threadIdx.x];
 }
 
 // One stable pass: items move to (items of smaller digits) + (items of the same
 // digit in earlier tiles) + (rank inside the tile).  FIRST reads the ids, later
 // passes the pairs.  next != NULL: counts the next digit per destination tile
 // (integer atomics: the counts do not depend on their order).
-template <bool FIRST>
-__global__ void __launch_bounds__(256) embed_scatter_kernel(SortIn in, const uint2* __restrict__ src, int64_t n_tokens,
+template <bool FIRST, int NW>
+__global__ void __launch_bounds__(NW * 32) embed_scatter_kernel(SortIn in, const uint2* __restrict__ src, int64_t n_tokens,
                                                             int64_t tile, int shift, const uint32_t* __restrict__ hist,
                                                             uint32_t* __restrict__ next, uint2* __restrict__ dst) {
-  __shared__ __align__(16) uint32_t cnt[8][256];
+  constexpr int kSubTile = NW * 32 * kRounds;
+  __shared__ __align__(16) uint32_t cnt[NW][256];
   __shared__ uint32_t total[256], base[256], warp_tot[8];
   // this block's items of the first sub-tile, on their way while the places are summed
   const int64_t lo = blockIdx.x * tile, hi = min(lo + tile, n_tokens);
@@ -381,28 +387,37 @@ __global__ void __launch_bounds__(256) embed_scatter_kernel(SortIn in, const uin
   };
   fetch(lo);
   {
-    // this tile's first place for every digit: four threads share a column of
-    // four digits, each takes every fourth tile
-    const int quad = threadIdx.x & 63, grp = threadIdx.x >> 6;
+    // this tile's first place for every digit: kParts threads share a column of
+    // four digits, each takes every kParts-th tile
+    constexpr int kParts = NW / 2;
+    const int quad = threadIdx.x & 63, part = threadIdx.x >> 6;
     const uint4* col = reinterpret_cast<const uint4*>(hist) + quad;
     const int tiles = gridDim.x, me = blockIdx.x;
     uint4 all = make_uint4(0u, 0u, 0u, 0u), before = all;
 #pragma unroll 8
-    for (int b = grp; b < tiles; b += 4) {
+    for (int b = part; b < tiles; b += kParts) {
       const uint4 c = __ldg(col + int64_t(b) * 64);
       const uint32_t m = b < me ? 0xffffffffu : 0u;
       all.x += c.x; all.y += c.y; all.z += c.z; all.w += c.w;
       before.x += c.x & m; before.y += c.y & m; before.z += c.z & m; before.w += c.w & m;
     }
-    *reinterpret_cast<uint4*>(&cnt[grp][quad * 4]) = all;
-    *reinterpret_cast<uint4*>(&cnt[4 + grp][quad * 4]) = before;
+    *reinterpret_cast<uint4*>(&cnt[part][quad * 4]) = all;
+    *reinterpret_cast<uint4*>(&cnt[kParts + part][quad * 4]) = before;
     __syncthreads();
     const int d = threadIdx.x;
-    total[d] = cnt[0][d] + cnt[1][d] + cnt[2][d] + cnt[3][d];
-    const uint32_t mine = cnt[4][d] + cnt[5][d] + cnt[6][d] + cnt[7][d];
+    uint32_t mine = 0;
+    if (d < 256) {
+      uint32_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        sum += cnt[i][d];
+        mine += cnt[kParts + i][d];
+      }
+      total[d] = sum;
+    }
     __syncthreads();
     scan256(total, base, warp_tot);
-    base[d] += mine;
+    if (d < 256) base[d] += mine;
     __syncthreads();
   }
   for (int64_t s0 = lo; s0 < hi; s0 += kSubTile) {
@@ -413,7 +428,7 @@ __global__ void __launch_bounds__(256) embed_scatter_kernel(SortIn in, const uin
       const int64_t n = s0 + warp_id() * (32 * kRounds) + i * 32 + lane_id();
       digit[i] = n < hi ? (key[i] >> shift) & 255u : 256u;
     }
-    rank_tile<8, kRounds>(digit, rank, cnt, total);
+    rank_tile<NW, kRounds>(digit, rank, cnt, total);
 #pragma unroll
     for (int i = 0; i < kRounds; ++i)
       if (digit[i] < 256) {
@@ -423,7 +438,7 @@ __global__ void __launch_bounds__(256) embed_scatter_kernel(SortIn in, const uin
           atomicAdd(&next[int64_t(at / (uint32_t)tile) * 256 + ((key[i] >> (shift + 8)) & 255u)], 1u);
       }
     __syncthreads();
-    base[threadIdx.x] += total[threadIdx.x];
+    if (threadIdx.x < 256) base[threadIdx.x] += total[threadIdx.x];
     __syncthreads();
   }
 }
@@ -847,8 +862,9 @@ EmbedPlan plan_embed(int64_t n, int64_t vocab, int64_t dim) {
   pl.bits = 1;
   while ((int64_t(1) << pl.bits) < vocab + 1) ++pl.bits;
   pl.passes = (pl.bits + 7) / 8;
-  pl.tile = kSubTile;
-  while ((n + pl.tile - 1) / pl.tile > kMaxTiles) pl.tile += kSubTile;
+  const int64_t sub_tile = sort_warps(n) * 32 * kRounds;
+  pl.tile = sub_tile;
+  while ((n + pl.tile - 1) / pl.tile > kMaxTiles) pl.tile += sub_tile;
   pl.tiles = (n + pl.tile - 1) / pl.tile;
   pl.chunk = n <= 32768 ? 32 : 64;
   pl.chunks = (n + pl.chunk - 1) / pl.chunk;
@@ -867,6 +883,26 @@ EmbedPlan plan_embed(int64_t n, int64_t vocab, int64_t dim) {
   at += up(pl.chunks * 2 * dim * 4);
   pl.bytes = at;
   return pl;
+}
+
+// Sort of more than kOneBlock tokens; pass p ends in pairs[p & 1].
+template <int NW>
+int sort_tiled(const SortIn& in, int64_t n, const EmbedPlan& pl, uint32_t* hist, uint2* seg, uint2* const (&pairs)[2],
+               cudaStream_t s) {
+  const unsigned grid = (unsigned)pl.tiles;
+  embed_hist_kernel<NW><<<grid, NW * 32, 0, s>>>(in, n, pl.tile, hist, pl.hist_words, seg);
+  int st = check_launch("embedding_bwd_hist");
+  for (int p = 0; st == MT_OK && p < pl.passes; ++p) {
+    const uint32_t* h = hist + int64_t(p) * pl.tiles * 256;
+    uint32_t* next = p + 1 < pl.passes ? hist + int64_t(p + 1) * pl.tiles * 256 : nullptr;
+    if (p == 0)
+      embed_scatter_kernel<true, NW><<<grid, NW * 32, 0, s>>>(in, nullptr, n, pl.tile, 0, h, next, pairs[0]);
+    else
+      embed_scatter_kernel<false, NW><<<grid, NW * 32, 0, s>>>(in, pairs[(p - 1) & 1], n, pl.tile, 8 * p, h, next,
+                                                               pairs[p & 1]);
+    st = check_launch("embedding_bwd_scatter");
+  }
+  return st;
 }
 
 int check_embed(int64_t n, int64_t vocab, int64_t dim) {
@@ -961,20 +997,9 @@ extern "C" int mt_embedding_bwd(const void* ids, int ids_i64, int64_t n, const v
     embed_sort_small_kernel<<<1, 1024, 0, s>>>(in, (int)n, pl.bits, sorted, seg);
     if ((st = check_launch("embedding_bwd_sort")) != MT_OK) return st;
   } else {
-    const unsigned grid = (unsigned)pl.tiles;
-    embed_hist_kernel<<<grid, 256, 0, s>>>(in, n, pl.tile, hist, pl.hist_words, seg);
-    if ((st = check_launch("embedding_bwd_hist")) != MT_OK) return st;
-    for (int p = 0; p < pl.passes; ++p) {
-      const uint32_t* h = hist + int64_t(p) * pl.tiles * 256;
-      uint32_t* next = p + 1 < pl.passes ? hist + int64_t(p + 1) * pl.tiles * 256 : nullptr;
-      uint2* dst = pairs[p & 1];
-      if (p == 0)
-        embed_scatter_kernel<true><<<grid, 256, 0, s>>>(in, nullptr, n, pl.tile, 0, h, next, dst);
-      else
-        embed_scatter_kernel<false><<<grid, 256, 0, s>>>(in, sorted, n, pl.tile, 8 * p, h, next, dst);
-      if ((st = check_launch("embedding_bwd_scatter")) != MT_OK) return st;
-      sorted = dst;
-    }
+    st = sort_warps(n) == 16 ? sort_tiled<16>(in, n, pl, hist, seg, pairs, s) : sort_tiled<8>(in, n, pl, hist, seg, pairs, s);
+    if (st != MT_OK) return st;
+    sorted = pairs[(pl.passes - 1) & 1];
   }
   return with_type(dout_dtype, [&](auto gv) {
     return with_type(dw_dtype, [&](auto dv) {
