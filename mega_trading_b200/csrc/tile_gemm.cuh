@@ -27,8 +27,8 @@
 // fp32 columns) of a warp's 32 rows.  They leave through the warp's own
 // 4 KB staging box and a TMA store (or TMA fp32 add), so no barrier spans
 // warps (32-byte stores straight from registers were 9 % slower, copying the box
-// out with 16-byte stores 17-30 %); outputs whose row stride or base is not a multiple of 16 bytes are
-// copied out of the box with plain coalesced stores.
+// out with 16-byte stores 17-30 %); outputs whose row stride or base is not a
+// multiple of 16 bytes are copied out of the box with plain coalesced stores.
 #pragma once
 
 #include <algorithm>
@@ -407,6 +407,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
 #pragma unroll 1
         for (int c = wg * kSpan; c < (wg + 1) * kSpan; c += 32) {
           uint32_t z[32];
+          __syncwarp();  // the TMEM loads want the whole warp
           tmem_ld32(acc + c, z);
           tmem_ld_wait();
           const int n0 = w.n0 + c;
@@ -418,6 +419,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
             const uint32_t asking = __ballot_sync(0xffffffffu, want < n0 + 32);
             if (asking == 0) break;
             const int col = __shfl_sync(0xffffffffu, want, __ffs(asking) - 1);
+            __syncwarp();
             const uint32_t v = tmem_ld1(acc + (col - w.n0));
             if (want == col) p.ep.take(st, v);
           }
@@ -457,6 +459,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
 #pragma unroll 1
         for (int c = wg; c < kSteps; c += kGroups) {
           uint32_t z[kSub][32];
+          __syncwarp();  // the TMEM loads want the whole warp
 #pragma unroll
           for (int h = 0; h < kSub; ++h) tmem_ld32(acc + c * kCols + h * 32, z[h]);
           tmem_ld_wait();
