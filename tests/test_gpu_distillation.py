@@ -334,3 +334,54 @@ def test_distillation_refuses_second_derivatives(cuda_device):
                                      torch.zeros(4, 1, device=cuda_device))
     with pytest.raises(RuntimeError, match="no second derivative"):
         torch.autograd.grad(loss, h, create_graph=True)
+
+
+def test_distillation_vocabulary_of_one(cuda_device):
+    """q is 1 everywhere: the loss and both gradients are zero."""
+    g = torch.Generator(device=cuda_device).manual_seed(10)
+    h = torch.randn(5, 8, device=cuda_device, generator=g).to(BF16)
+    w = torch.randn(1, 8, device=cuda_device, generator=g).to(BF16)
+    ids = torch.zeros(5, 3, dtype=torch.long, device=cuda_device)
+    logits = torch.zeros(5, 3, device=cuda_device)
+    # three equal entries of one id: p = 1 after merging, each entry counts its own log(1/3)
+    loss, dh, dw = _run(cuda_device, h, w, ids, logits, 1.0, BF16)
+    _check(h, w, ids, logits, 1.0, BF16, 1.0, loss, dh, dw)
+    loss, dh, dw = _run(cuda_device, h, w, ids[:, :1], logits[:, :1], 1.0, BF16)
+    assert abs(float(loss)) <= 1e-4 and float(dh.abs().max()) <= 1e-4 and float(dw.abs().max()) <= 1e-4
+
+
+def test_distillation_nan_hidden_row_reaches_the_loss(cuda_device):
+    g = torch.Generator(device=cuda_device).manual_seed(11)
+    h = torch.randn(6, 64, device=cuda_device, generator=g).to(BF16)
+    w = (torch.randn(90, 64, device=cuda_device, generator=g) * 0.1).to(BF16)
+    ids, logits = _teacher(6, 90, 4, 11, cuda_device)
+    bad = h.clone()
+    bad[2, 5] = float("nan")
+    loss, dh, _ = _run(cuda_device, bad, w, ids, logits, 1.0, BF16)
+    assert bool(loss.isnan()) and bool(dh[2].isnan().all()) and bool(dh[[0, 1, 3, 4, 5]].isfinite().all())
+
+
+def test_distillation_calls_on_two_streams_do_not_mix(cuda_device):
+    g = torch.Generator(device=cuda_device).manual_seed(12)
+    w = (torch.randn(3000, 256, device=cuda_device, generator=g) * 0.1).to(BF16)
+    cases = []
+    for i in range(4):
+        h = torch.randn(700 + 300 * i, 256, device=cuda_device, generator=g).to(BF16)
+        cases.append((h, *_teacher(h.shape[0], 3000, 10, 20 + i, cuda_device)))
+    want = [_run(cuda_device, h, w, ids, lg, 1.5, BF16) for h, ids, lg in cases]
+    torch.cuda.synchronize()
+    from mega_trading_b200.kernels.distillation import fused_linear_distillation
+
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for s, (h, ids, lg) in zip(streams, cases):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            hd, wd = h.clone().requires_grad_(), w.clone().requires_grad_()
+            loss = fused_linear_distillation(hd, wd, ids, lg, temperature=1.5)
+            got.append((loss.detach(), *torch.autograd.grad(loss, (hd, wd))))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -252,3 +252,24 @@ def test_embedding_gradient_off_the_vector_grid(cuda_device, n):
     g = torch.randn(n * 64 + 1, device=cuda_device, generator=gen)[1:].view(n, 64)
     (dw,) = torch.autograd.grad(scaled_embedding(ids, w), w, g)
     _check_grad(dw, ids, g, 60, 1.0, None)
+
+
+def test_embedding_calls_on_two_streams_do_not_mix(cuda_device):
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    gen = torch.Generator(device=cuda_device).manual_seed(8)
+    cases = [(torch.randint(0, 4000, (n,), device=cuda_device, generator=gen),
+              torch.randn(4000, 96, device=cuda_device, generator=gen, requires_grad=True),
+              torch.randn(n, 96, device=cuda_device, generator=gen)) for n in (100, 1500, 9000, 80000)]
+    want = [torch.autograd.grad(scaled_embedding(i, w), w, g)[0] for i, w, g in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], []
+    for s, (i, w, g) in zip(streams, cases):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            leaf = w.detach().requires_grad_()
+            got.append(torch.autograd.grad(scaled_embedding(i, leaf), leaf, g)[0])
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

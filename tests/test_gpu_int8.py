@@ -268,3 +268,20 @@ def test_int8_linear_on_another_stream_and_in_a_graph(cuda_device):
     torch.cuda.synchronize()
     assert torch.equal(out, step())
     assert not torch.equal(out, want)
+
+
+def test_int8_nan_scale_reaches_the_product(cuda_device):
+    """A row with an infinity or NaN quantises to a NaN scale, and its products are NaN, alone."""
+    from mega_trading_b200.kernels import int8
+
+    gen = torch.Generator(device=cuda_device).manual_seed(7)
+    wq, ws = int8.quantize_rows_int8(torch.randn(300, 64, device=cuda_device, generator=gen))
+    for rows in (5, 140):
+        x = torch.randn(rows, 64, device=cuda_device, generator=gen)
+        x[1, 3], x[3, 0] = float("inf"), float("nan")
+        q, s = int8.quantize_rows_int8(x)
+        y = int8.int8_linear(q, s, wq, ws)
+        assert bool(y[[1, 3]].isnan().all())
+        keep = torch.ones(rows, dtype=torch.bool, device=cuda_device)
+        keep[[1, 3]] = False
+        assert bool(y[keep].isfinite().all())
