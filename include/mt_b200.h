@@ -379,10 +379,10 @@ MT_API int mt_distill_fwd(const void* hidden, const void* weight, int dtype,
                           void* stream);
 
 /* Backward: dz = (q - p) * temperature * grad_out / rows;  dhidden = dz weight,
- * dweight = dz^T hidden.  dz is rounded to dtype (once, after the subtraction)
- * and exists for one chunk of rows at a time in the workspace
- * (mt_distill_bwd_workspace_bytes(), 256-byte aligned: at most 256 MB of dz
- * plus fp32 partial sums); sums are fp32 in a fixed order.  grad_out: device
+ * dweight = dz^T hidden.  dz is rounded to dtype (once, after the subtraction;
+ * a call of one or two rows may keep it in fp32) and exists for one chunk of
+ * rows at a time in the workspace (mt_distill_bwd_workspace_bytes(), 256-byte
+ * aligned: at most 256 MB of dz plus fp32 partial sums); sums are fp32 in a fixed order.  grad_out: device
  * fp32 scalar.  dhidden [N, K] / dweight [V, K] contiguous, 16-byte aligned,
  * in dh_dtype / dw_dtype; either may be NULL to skip it. */
 MT_API int64_t mt_distill_bwd_workspace_bytes(int64_t N, int64_t V, int64_t K);

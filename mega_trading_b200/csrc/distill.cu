@@ -28,7 +28,8 @@
 // fp32: it would push 16-bit values of a mean over many rows out of range.
 // fp16 values are held times 2^15 for the same reason (|q - p| <= 1).  The rounding of
 // dz to 16 bits (half a step of its own magnitude) is the tensor cores' operand
-// type and the one rounding between the fp32 logits and the fp32 sums.
+// type and the one rounding between the fp32 logits and the fp32 sums.  One or
+// two rows take a path without tiles or that rounding.
 //
 // Bound by the tensor pipe and, in a steady stream, by the power limit: 32,768
 // rows x 768 against 21,504 entries, forward and backward, 3.86 ms (8 NVK
@@ -424,6 +425,191 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict
 }
 
 // ---------------------------------------------------------------------------
+// backward of a few rows: everything in fp32, no tiles
+// ---------------------------------------------------------------------------
+// With up to kFewRows rows a 256-row tile would be nearly empty and W is what
+// there is to read, so two passes over it do: one warp per vocabulary entry v
+// forms the rows' z_v by dot products, dz_v = q - p and dW_v = sum_r dz_rv h_r at
+// once; then dh = dz W in strips of v, joined in a fixed order.  dz stays in fp32
+// (a single row's error would otherwise be one rounding of its largest entry).
+// Measured against the tiles, backward alone, cold cache: 21,504 x 768, 1 row 31
+// against 49 us and 2 rows 39 against 51; 2,048 columns, 68 against 92 and 84
+// against 94; 2,000 x 256, 12 against 29.  Past the L2 the second pass over W pays
+// HBM again: 100,000 x 1,024, 178 against 158.  The dot products of more rows cost
+// instructions (an earlier form: 4 rows of 2,048 columns 109 against 88).
+constexpr int kFewRows = 2;
+constexpr int kFewK = 2048;  // and the rows' hidden states in 8 KB of shared memory
+constexpr int64_t kFewWeight = 64 << 20;  // V * K: 128 MB, about the L2
+constexpr int kFewStrips = 512;
+
+struct FewParams {
+  const void* hidden;
+  const void* weight;
+  int N, V, K, top;
+  float zscale, factor;  // log2(e) / temperature, temperature
+  const int* tid;
+  const float* tp;
+  const float* lse2;
+  const float* inv_rows;
+  const float* grad_out;
+  float* dz;  // [N, V] fp32
+  void* dw;   // may be NULL
+};
+
+// p of id v in a row's list (rising ids, kNone past the last).
+__device__ __forceinline__ float listed_prob(const int* tid, const float* tp, int top, int v) {
+  int lo = 0, hi = top;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(tid + mid) < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo < top && __ldg(tid + lo) == v ? __ldg(tp + lo) : 0.f;
+}
+
+template <typename T, typename TO, int MT>
+__global__ void __launch_bounds__(256) distill_few_dw_kernel(const FewParams p) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  T* h = reinterpret_cast<T*>(raw);  // [N, K]
+  const int lane = lane_id();
+  for (int i = threadIdx.x * 8; i < p.N * p.K; i += 256 * 8)
+    *reinterpret_cast<uint4*>(h + i) = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.hidden) + i));
+  __syncthreads();
+  const float lse2 = lane < p.N ? __ldg(p.lse2 + lane) : INFINITY;
+  const float g = p.factor * __ldg(p.grad_out) * __ldg(p.inv_rows);
+  const int warps = gridDim.x * 8;
+  for (int v = blockIdx.x * 8 + warp_id(); v < p.V; v += warps) {
+    const T* wv = static_cast<const T*>(p.weight) + int64_t(v) * p.K;
+    float z[MT];
+#pragma unroll
+    for (int r = 0; r < MT; ++r) z[r] = 0.f;
+#pragma unroll 4
+    for (int k = lane * 8; k < p.K; k += 256) {
+      float x[8];
+      load_vec<T, 8>(wv + k, x);
+#pragma unroll
+      for (int r = 0; r < MT; ++r)
+        if (r < p.N) {
+          float y[8];
+          load_vec<T, 8>(h + r * p.K + k, y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) z[r] = fmaf(x[e], y[e], z[r]);
+        }
+    }
+    float mine = 0.f;  // lane r: row r's logit
+#pragma unroll
+    for (int r = 0; r < MT; ++r) {
+      const float t = warp_sum(z[r]);
+      if (lane == r) mine = t;
+    }
+    float d = 0.f;
+    if (lane < p.N && lse2 != INFINITY) {  // rows without an entry stay out
+      d = exp2f(fmaf(mine, p.zscale, -lse2)) - listed_prob(p.tid + lane * p.top, p.tp + lane * p.top, p.top, v);
+    }
+    if (lane < p.N) p.dz[int64_t(lane) * p.V + v] = d;
+    if (p.dw != nullptr) {
+      TO* out = static_cast<TO*>(p.dw) + int64_t(v) * p.K;
+      for (int k0 = 0; k0 < p.K; k0 += 256) {
+        const int k = k0 + lane * 8;
+        float acc[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+        for (int r = 0; r < p.N; ++r) {
+          const float dr = __shfl_sync(0xffffffffu, d, r);
+          if (dr != 0.f && k < p.K) {
+            float y[8];
+            load_vec<T, 8>(h + r * p.K + k, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = fmaf(dr, y[e], acc[e]);
+          }
+        }
+        if (k < p.K) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] *= g;
+          if constexpr (sizeof(TO) == 2) {
+            store_vec<TO, 8>(out + k, acc);
+          } else {
+            store_vec<TO, 4>(out + k, {acc[0], acc[1], acc[2], acc[3]});
+            store_vec<TO, 4>(out + k + 4, {acc[4], acc[5], acc[6], acc[7]});
+          }
+        }
+      }
+    }
+  }
+}
+
+// A strip of vocabulary entries for 256 columns (two per thread): partial sums
+// part[strip, r, k] of dz W.
+template <typename T, int MT>
+__global__ void __launch_bounds__(128) distill_few_dh_kernel(const float* __restrict__ dz, const T* __restrict__ w,
+                                                             int N, int V, int K, int strip,
+                                                             float* __restrict__ part) {
+  __shared__ float s[MT][64];
+  const int k = blockIdx.y * 256 + threadIdx.x * 2;
+  const int lo = blockIdx.x * strip, hi = min(lo + strip, V);
+  float2 acc[MT];
+#pragma unroll
+  for (int r = 0; r < MT; ++r) acc[r] = make_float2(0.f, 0.f);
+  for (int v0 = lo; v0 < hi; v0 += 64) {
+    const int nv = min(64, hi - v0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 64; i += 128) {
+      const int r = i >> 6, j = i & 63;
+      s[r][j] = r < N && j < nv ? dz[int64_t(r) * V + v0 + j] : 0.f;
+    }
+    __syncthreads();
+    if (k >= K) continue;
+    const T* wp = w + int64_t(v0) * K + k;
+    for (int j0 = 0; j0 < nv; j0 += 8) {
+      uint32_t x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        x[j] = j0 + j < nv ? __ldg(reinterpret_cast<const uint32_t*>(wp + int64_t(j0 + j) * K)) : 0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float a, b;
+        unpack2<T>(x[j], a, b);
+#pragma unroll
+        for (int r = 0; r < MT; ++r) {
+          acc[r].x = fmaf(s[r][j0 + j], a, acc[r].x);
+          acc[r].y = fmaf(s[r][j0 + j], b, acc[r].y);
+        }
+      }
+    }
+  }
+  if (k >= K) return;
+#pragma unroll
+  for (int r = 0; r < MT; ++r)
+    if (r < N) *reinterpret_cast<float2*>(part + (int64_t(blockIdx.x) * N + r) * K + k) = acc[r];
+}
+
+// dh = factor * sum over strips (8 lanes of strips per element, then in order).
+template <typename TO>
+__global__ void __launch_bounds__(256) distill_few_join_kernel(const float* __restrict__ part, int strips, int n,
+                                                               float factor, const float* __restrict__ inv_rows,
+                                                               const float* __restrict__ grad_out,
+                                                               TO* __restrict__ out) {
+  __shared__ float s[8][32];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int i = blockIdx.x * 32 + x;
+  float a = 0.f;
+  if (i < n) {
+#pragma unroll 8
+    for (int q = y; q < strips; q += 8) a += part[int64_t(q) * n + i];
+  }
+  s[y][x] = a;
+  __syncthreads();
+  if (y == 0 && i < n) {
+    float t = s[0][x];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) t += s[q][x];
+    out[i] = from_f32<TO>(t * (factor * __ldg(grad_out) * __ldg(inv_rows)));
+  }
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -713,6 +899,53 @@ int run_bwd(const BwdArgs& a, const BwdPlan& pl) {
   return MT_OK;
 }
 
+bool few_rows(int64_t N, int64_t V, int64_t K) { return N <= kFewRows && K <= kFewK && V * K <= kFewWeight; }
+int64_t few_part_off(int64_t N, int64_t V) { return up256(N * V * 4); }
+int64_t few_bytes(int64_t N, int64_t V, int64_t K) { return few_part_off(N, V) + up256(kFewStrips * N * K * 4); }
+
+template <typename T, typename TO, int MT>
+int launch_few_dw(const FewParams& p, cudaStream_t s) {
+  auto kern = distill_few_dw_kernel<T, TO, MT>;
+  const int smem = p.N * p.K * (int)sizeof(T);
+  const int grid = (int)std::min<int64_t>((int64_t(p.V) + 7) / 8, int64_t(get_sm_count()) * 8);
+  kern<<<grid, 256, smem, s>>>(p);
+  return check_launch("distill_bwd_few_dw");
+}
+
+template <typename T, int MT>
+int run_few_rows(const BwdArgs& a) {
+  float* dz = reinterpret_cast<float*>(a.ws);
+  float* part = reinterpret_cast<float*>(a.ws + few_part_off(a.N, a.V));
+  const FewParams p{a.hidden, a.weight, (int)a.N, (int)a.V, (int)a.K, a.top, kLog2e / a.temp, a.temp, a.tid, a.tp,
+                    a.lse2, a.inv_rows, a.grad_out, dz, a.dw};
+  int st = a.dw_dtype == MT_F32    ? launch_few_dw<T, float, MT>(p, a.s)
+           : a.dw_dtype == MT_BF16 ? launch_few_dw<T, __nv_bfloat16, MT>(p, a.s)
+                                   : launch_few_dw<T, __half, MT>(p, a.s);
+  if (st != MT_OK || a.dh == nullptr) return st;
+  const int strip = std::max(16, (int)((a.V + kFewStrips - 1) / kFewStrips)), strips = (int)((a.V + strip - 1) / strip);
+  distill_few_dh_kernel<T, MT><<<dim3((unsigned)strips, (unsigned)((a.K + 255) / 256)), 128, 0, a.s>>>(
+      dz, static_cast<const T*>(a.weight), (int)a.N, (int)a.V, (int)a.K, strip, part);
+  if ((st = check_launch("distill_bwd_few_dh")) != MT_OK) return st;
+  const int n = (int)(a.N * a.K);
+  const unsigned grid = (unsigned)((n + 31) / 32);
+  if (a.dh_dtype == MT_F32)
+    distill_few_join_kernel<float><<<grid, 256, 0, a.s>>>(part, strips, n, a.temp, a.inv_rows, a.grad_out,
+                                                          static_cast<float*>(a.dh));
+  else if (a.dh_dtype == MT_BF16)
+    distill_few_join_kernel<__nv_bfloat16><<<grid, 256, 0, a.s>>>(part, strips, n, a.temp, a.inv_rows, a.grad_out,
+                                                                  static_cast<__nv_bfloat16*>(a.dh));
+  else
+    distill_few_join_kernel<__half><<<grid, 256, 0, a.s>>>(part, strips, n, a.temp, a.inv_rows, a.grad_out,
+                                                           static_cast<__half*>(a.dh));
+  return check_launch("distill_bwd_few_join");
+}
+
+template <typename T>
+int run_few(const BwdArgs& a) {
+  if (a.N == 1) return run_few_rows<T, 1>(a);
+  return run_few_rows<T, kFewRows>(a);
+}
+
 int check_args(const void* hidden, const void* weight, int dtype, int64_t N, int64_t V, int64_t K, int64_t top,
                float temp) {
   if (dtype != MT_BF16 && dtype != MT_F16) return MT_ERR_UNSUPPORTED_DTYPE;
@@ -792,7 +1025,7 @@ extern "C" int mt_distill_fwd(const void* hidden, const void* weight, int dtype,
 
 extern "C" int64_t mt_distill_bwd_workspace_bytes(int64_t N, int64_t V, int64_t K) {
   if (N <= 0 || V <= 0 || K <= 0) return 256;
-  return plan_bwd(N, V, K).bytes;
+  return few_rows(N, V, K) ? few_bytes(N, V, K) : plan_bwd(N, V, K).bytes;
 }
 
 extern "C" int mt_distill_bwd(const void* hidden, const void* weight, int dtype, int64_t N, int64_t V, int64_t K,
@@ -815,13 +1048,16 @@ extern "C" int mt_distill_bwd(const void* hidden, const void* weight, int dtype,
   if (list_ids == nullptr || list_probs == nullptr || list_logits == nullptr || row_stats == nullptr ||
       grad_out == nullptr || status == nullptr)
     return MT_ERR_INVALID_ARGUMENT;
+  const bool few = few_rows(N, V, K);
   const BwdPlan pl = plan_bwd(N, V, K);
-  if (workspace == nullptr || !aligned_to(workspace, 256) || workspace_bytes < pl.bytes) return MT_ERR_WORKSPACE;
+  if (workspace == nullptr || !aligned_to(workspace, 256) || workspace_bytes < mt_distill_bwd_workspace_bytes(N, V, K))
+    return MT_ERR_WORKSPACE;
   if (std::max(pl.h_splits, pl.h_last) * pl.h_pad > 0x7fffffffLL || pl.w_splits * pl.w_pad > 0x7fffffffLL) return MT_ERR_INVALID_ARGUMENT;
   if ((st = bind_device_of(hidden)) != MT_OK) return st;
   if ((st = check_arch()) != MT_OK) return st;
   const BwdArgs a{hidden, weight, N, V, K, (int)top, temperature, list_ids, list_probs, list_logits, row_stats,
                   row_stats + N + 2, grad_out, dhidden, dh_dtype, dweight, dw_dtype, static_cast<char*>(workspace),
                   status, s};
+  if (few) return dtype == MT_BF16 ? run_few<__nv_bfloat16>(a) : run_few<__half>(a);
   return dtype == MT_BF16 ? run_bwd<__nv_bfloat16, kKindBf16>(a, pl) : run_bwd<__half, kKindF16>(a, pl);
 }

@@ -93,6 +93,14 @@ def _teacher(n, v, top, seed, dev, masked=0.0, empty=0.0):
 
 @pytest.mark.parametrize("n,v,k,top,temp,dtype,masked,seed", [
     (1, 21504, 768, 8, 1.0, BF16, 0.0, 1),        # one token
+    (1, 500, 1032, 1, 0.7, F16, 0.0, 13),
+    (2, 1001, 64, 4, 1.0, BF16, 0.3, 14),
+    (2, 21504, 768, 32, 2.0, F16, 0.2, 15),       # the most rows without tiles
+    (2, 97, 2048, 9, 1.0, BF16, 0.2, 16),         # and the widest
+    (2, 300, 2056, 5, 1.0, BF16, 0.0, 17),        # too wide for them
+    (1, 70000, 1024, 3, 1.0, BF16, 0.0, 20),      # too large a weight
+    (3, 2000, 256, 8, 1.0, BF16, 0.1, 18),        # the fewest rows in tiles
+    (16, 21504, 768, 32, 2.0, F16, 0.2, 19),
     (300, 17, 64, 5, 2.0, BF16, 0.2, 2),          # a small vocabulary
     (77, 1000, 8, 1, 1.0, F16, 0.0, 3),           # the narrowest projection, one listed entry
     (130, 129, 104, 128, 0.5, BF16, 0.1, 4),
@@ -385,3 +393,18 @@ def test_distillation_calls_on_two_streams_do_not_mix(cuda_device):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("n", [1, 2])
+def test_distillation_of_few_rows_keeps_dz_in_fp32(cuda_device, n):
+    """No 16-bit rounding of dz: fp32 gradients within the sums' own rounding of the definition."""
+    g = torch.Generator(device=cuda_device).manual_seed(n)
+    h = torch.randn(n, 128, device=cuda_device, generator=g).to(BF16).float()
+    w = (torch.randn(700, 128, device=cuda_device, generator=g) * 0.1).to(BF16).float()
+    ids, logits = _teacher(n, 700, 6, n, cuda_device)
+    _, dh, dw = _run(cuda_device, h, w, ids, logits, 1.5, BF16)
+    _, dz, q, rows = _definition(h.double(), w.double(), ids, logits, 1.5)
+    for got, want, mag in ((dh, dz @ w.double(), dz.abs() @ w.double().abs()),
+                           (dw, dz.t() @ h.double(), dz.abs().t() @ h.double().abs())):
+        # q carries the error of its logit and of the row's sum, 1e-5 relative and more than covered by 1e-4
+        assert bool(((got.double() - 1.5 / rows * want).abs() <= 1.5 / rows * 1e-4 * (mag + 1e-6)).all())
