@@ -591,13 +591,18 @@ __global__ void __launch_bounds__(kBulkThreads) embed_reduce_bulk_kernel(
       prev = __shfl_sync(0xffffffffu, mine.x, 31);
       for (int g = 0; g < 32 && b0 + g < hi; g += rp, ++it) {
         const int st = it % kBulkStages;
-        if (it >= kBulkStages && !wait_bounded(wc, &sm.empty[st], ((it / kBulkStages) & 1) ^ 1, 1)) {
+        // every lane waits, and the warp leaves together when one of them gives up
+        if (it >= kBulkStages &&
+            !__all_sync(0xffffffffu, wait_bounded(wc, &sm.empty[st], ((it / kBulkStages) & 1) ^ 1, 1))) {
           ok = false;
           break;
         }
         const bool here = lane >= g && lane < g + rp;
         if (here) sm.meta[st][lane - g] = make_uint2(mine.x, flags);
         const uint32_t n = __popc(__ballot_sync(0xffffffffu, here && row));
+        // lane 0's arrival releases the other lanes' entries too (a stage without
+        // rows is complete with it)
+        __syncwarp();
         if (lane == 0) {
           if (n > 0)
             mbar_arrive_expect_tx(&sm.full[st], n * bytes);
@@ -610,7 +615,6 @@ __global__ void __launch_bounds__(kBulkThreads) embed_reduce_bulk_kernel(
       }
       mine = b0 + 32 + lane < hi ? later : make_uint2(0xffffffffu, 0u);
     }
-    ok = __all_sync(0xffffffffu, ok);
     if (!ok || sm.abort_flag) {
       for (int j = (it > kBulkStages ? it - kBulkStages : 0); j < it; ++j)
         wait_drain(wc, &sm.full[j % kBulkStages], (j / kBulkStages) & 1, 11);
@@ -626,7 +630,7 @@ __global__ void __launch_bounds__(kBulkThreads) embed_reduce_bulk_kernel(
     int64_t at = lo;
     for (int it = 0; at < hi; ++it) {
       const int st = it % kBulkStages;
-      if (!wait_bounded(wc, &sm.full[st], (it / kBulkStages) & 1, 2)) break;
+      if (!__all_sync(0xffffffffu, wait_bounded(wc, &sm.full[st], (it / kBulkStages) & 1, 2))) break;
       const int rows = (int)min((int64_t)rp, hi - at);
       // four rows at a time: their values and run flags are fetched together
       for (int i0 = 0; i0 < rows; i0 += 4) {

@@ -273,3 +273,29 @@ def test_embedding_calls_on_two_streams_do_not_mix(cuda_device):
         torch.cuda.current_stream().wait_stream(s)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("n,dim,ot,share", [
+    (9000, 1024, F32, 0.7),    # four rows to a stage of the gather ring: most stages hold no row
+    (30000, 96, BF16, 0.5),    # 32 rows to a stage
+    (3000, 2048, BF16, 1.0),   # no row anywhere
+])
+def test_embedding_gradient_with_ranges_of_padding_only(cuda_device, n, dim, ot, share):
+    """Padded places sort last: whole ranges of the sorted order without a row to add.  What the
+    ring held before must not reach the sums, every time."""
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    g = torch.Generator(device=cuda_device).manual_seed(n)
+    vocab, pad = 700, 13
+    ids = torch.randint(0, vocab, (n,), device=cuda_device, generator=g)
+    gone = torch.rand(n, device=cuda_device, generator=g) < share
+    ids[gone] = pad
+    ids[~gone & (ids == pad)] = pad + 1
+    w = torch.randn(vocab, dim, device=cuda_device, generator=g).to(ot).requires_grad_()
+    grad = torch.randn(n, dim, device=cuda_device, generator=g).to(ot)
+    (first,) = torch.autograd.grad(scaled_embedding(ids, w, padding_idx=pad), w, grad)
+    _check_grad(first, ids, grad, vocab, 1.0, pad)
+    grad[gone] = float("nan")
+    for _ in range(8):
+        (again,) = torch.autograd.grad(scaled_embedding(ids, w, padding_idx=pad), w, grad)
+        assert torch.equal(again, first)
