@@ -219,14 +219,16 @@ struct StatsEpilogue {
 #pragma unroll
     for (int i = 2; i < 32; i += 2) cm = fmax3(cm, x[i], x[i + 1]);
     const float mn = fmaxf(st.m, cm * zscale);  // zscale > 0
-    const float2 zs = make_float2(zscale, zscale), sh = make_float2(-mn, -mn);
+    // a maximum of -inf means nothing but -inf (which adds 0) or NaN (which has to stay) so far
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float2 zs = make_float2(zscale, zscale), sh = make_float2(-base, -base);
     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       const float2 e = fma2(make_float2(x[i], x[i + 1]), zs, sh);
       sum = add2(sum, make_float2(fast_exp2(e.x), fast_exp2(e.y)));
     }
-    st.s = (st.m == -INFINITY ? 0.f : st.s * fast_exp2(st.m - mn)) + (sum.x + sum.y);
+    st.s = st.s * fast_exp2(st.m - base) + (sum.x + sum.y);
     st.m = mn;
   }
   __device__ __forceinline__ void end(const State& st) const {
@@ -268,9 +270,10 @@ __global__ void __launch_bounds__(256) distill_row_kernel(const RowParams p) {
     float M = -INFINITY;
     for (int i = lane; i < used; i += 32) M = fmaxf(M, pm[i]);
     M = warp_max(M);
+    const float base = M == -INFINITY ? 0.f : M;
     float S = 0.f;
-    for (int i = lane; i < used; i += 32) S += pm[i] == -INFINITY ? 0.f : ps[i] * exp2f(pm[i] - M);
-    const float l2 = M + log2f(warp_sum(S));
+    for (int i = lane; i < used; i += 32) S += ps[i] * exp2f(pm[i] - base);  // pm -inf: ps is 0 or NaN
+    const float l2 = base + log2f(warp_sum(S));
     const bool live = p.mass[row] != 0.f;
     if (live) {
       float cross = 0.f;

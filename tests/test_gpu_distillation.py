@@ -408,3 +408,29 @@ def test_distillation_of_few_rows_keeps_dz_in_fp32(cuda_device, n):
                            (dw, dz.t() @ h.double(), dz.abs().t() @ h.double().abs())):
         # q carries the error of its logit and of the row's sum, 1e-5 relative and more than covered by 1e-4
         assert bool(((got.double() - 1.5 / rows * want).abs() <= 1.5 / rows * 1e-4 * (mag + 1e-6)).all())
+
+
+@pytest.mark.parametrize("lo,n", [(0, 5), (64, 5), (384, 300), (0, 1)])
+def test_distillation_nan_weight_rows_reach_the_loss(cuda_device, lo, n):
+    """32 neighbouring NaN rows of the weight: every logit of the first step a thread looks at."""
+    g = torch.Generator(device=cuda_device).manual_seed(13)
+    h = torch.randn(n, 64, device=cuda_device, generator=g).to(BF16)
+    w = (torch.randn(900, 64, device=cuda_device, generator=g) * 0.1).to(BF16)
+    w[lo:lo + 32] = float("nan")
+    ids = torch.tensor([[800, 700]], device=cuda_device).expand(n, 2)
+    loss, _, _ = _run(cuda_device, h, w, ids, torch.zeros(n, 2, device=cuda_device), 1.0, BF16)
+    assert bool(loss.isnan())
+
+
+def test_distillation_entries_of_no_probability_leave_the_loss(cuda_device):
+    """Vocabulary entries whose logits are -inf, whole steps and pieces of them, are entries with q = 0."""
+    g = torch.Generator(device=cuda_device).manual_seed(14)
+    h = (torch.rand(5, 64, device=cuda_device, generator=g) + 0.5).to(BF16)
+    w = (torch.randn(900, 64, device=cuda_device, generator=g) * 0.1).to(BF16)
+    w[0:64] = w[300:600] = -float("inf")
+    ids = torch.tensor([[800, 700]], device=cuda_device).expand(5, 2)
+    logits = torch.zeros(5, 2, device=cuda_device)
+    loss, _, _ = _run(cuda_device, h, w, ids, logits, 1.0, BF16)
+    ref = _definition(h.double(), w.double(), ids, logits, 1.0)[0]
+    # the module's bound; |h| |w| <= 12 for the finite rows
+    assert abs(float(loss) - float(ref)) <= 2 * (64 / 16 + 4) * 2.0 ** -23 * 12 + 1e-4
