@@ -382,8 +382,9 @@ MT_API int mt_distill_fwd(const void* hidden, const void* weight, int dtype,
  * dweight = dz^T hidden.  dz is rounded to dtype (once, after the subtraction;
  * a call of one or two rows may keep it in fp32) and exists for one chunk of
  * rows at a time in the workspace (mt_distill_bwd_workspace_bytes(), 256-byte
- * aligned: at most 256 MB of dz plus fp32 partial sums); sums are fp32 in a fixed order.  grad_out: device
- * fp32 scalar.  dhidden [N, K] / dweight [V, K] contiguous, 16-byte aligned,
+ * aligned: at most 256 MB of dz, the chunk's hidden states and fp32 partial sums);
+ * sums are fp32 in a fixed order.  Rows without an entry add nothing whatever their
+ * hidden states hold.  grad_out: device fp32 scalar.  dhidden [N, K] / dweight [V, K] contiguous, 16-byte aligned,
  * in dh_dtype / dw_dtype; either may be NULL to skip it. */
 MT_API int64_t mt_distill_bwd_workspace_bytes(int64_t N, int64_t V, int64_t K);
 MT_API int mt_distill_bwd(const void* hidden, const void* weight, int dtype, int64_t N, int64_t V,

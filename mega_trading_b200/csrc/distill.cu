@@ -23,7 +23,8 @@
 //   2. listed entries are overwritten with round(q - p) from the forward's
 //      fp32 logits: the difference is rounded once, not its parts
 //   3. dh chunk = dz W        (W read along its rows, no transposed copy)
-//   4. dW      += dz^T h      (fp32, both operands read along their rows)
+//   4. dW      += dz^T h      (fp32, both operands read along their rows; rows
+//      without an entry as zeros whatever they hold: 0 * inf is NaN)
 // q - p is kept without the factor T * grad / n, which the epilogues apply in
 // fp32: it would push 16-bit values of a mean over many rows out of range.
 // fp16 values are held times 2^15 for the same reason (|q - p| <= 1).  The rounding of
@@ -175,6 +176,7 @@ struct StatsEpilogue {
   static constexpr uint32_t kKernelId = mt::kKernelId;
   static constexpr int OUT_SIZE = 4;
   static constexpr bool kStats = true;
+  static constexpr bool kAltB = false;
   const int* tid;
   float* zt;
   float* part_m;  // [N, pieces]: pieces = slots * groups
@@ -341,6 +343,7 @@ struct SoftmaxEpilogue {
   static constexpr uint32_t kKernelId = mt::kKernelId;
   static constexpr int OUT_SIZE = 2;
   static constexpr bool kStats = false;
+  static constexpr bool kAltB = false;
   const float* lse2;
   float zscale;
   float log2_up;
@@ -364,16 +367,32 @@ struct SoftmaxEpilogue {
   }
 };
 
+// The hidden states that dW's product reads: rows without an entry have dz = 0,
+// but 0 times an infinity or a NaN is NaN, so where such rows exist the product
+// reads a copy of the chunk in which they are zero.
+struct LiveHidden {
+  CUtensorMap copy;
+  const float* live;  // rows with an entry in the whole batch
+  float rows;         // fewer than this many: read the copy
+};
+struct NoOther {};
+
 // accumulator * temp * grad_out / rows / up
-template <typename TO>
+template <typename TO, bool DW>
 struct GradEpilogue {
   static constexpr uint32_t kKernelId = mt::kKernelId;
   static constexpr int OUT_SIZE = sizeof(TO);
   static constexpr bool kStats = false;
+  static constexpr bool kAltB = DW;
   const float* inv_rows;
   const float* grad_out;
   float factor;  // temp / up
   bool add, direct;
+  typename std::conditional<DW, LiveHidden, NoOther>::type hidden;
+
+  __device__ __forceinline__ const CUtensorMap* b_map(const CUtensorMap* all) const {
+    return __ldg(hidden.live) < hidden.rows ? &hidden.copy : all;
+  }
 
   struct Row {
     float g;
@@ -392,19 +411,46 @@ struct GradEpilogue {
   }
 };
 
-// Listed entries of a chunk of rows: dz = round((q - p) * up).
+// Listed entries of a chunk of rows: dz = round((q - p) * up); and, in the blocks
+// after those, the chunk's hidden states with zero rows where there is no entry
+// (none to write when every row of the batch has one).
+struct ListedParams {
+  const int* tid;
+  const float *tp, *zt, *lse2;
+  uint32_t n, top;        // entries in all, per row
+  unsigned entry_blocks;  // blocks for them
+  float zscale, up;
+  void* dz;
+  int64_t ld;
+  const uint4* hidden;
+  uint4* copy;
+  int rows, words;        // of the chunk, 16-byte words of a row
+  const float* live;      // as in LiveHidden
+  float all_rows;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256) distill_listed_kernel(const int* __restrict__ tid, const float* __restrict__ tp,
-                                                             const float* __restrict__ zt,
-                                                             const float* __restrict__ lse2, uint32_t n, uint32_t top,
-                                                             float zscale, float up, T* __restrict__ dz, int64_t ld) {
+__global__ void __launch_bounds__(256) distill_listed_kernel(const ListedParams p) {
+  if (blockIdx.x >= p.entry_blocks) {
+    if (!(__ldg(p.live) < p.all_rows)) return;
+    // a warp per row
+    const int step = (gridDim.x - p.entry_blocks) * 8;
+    for (int r = (blockIdx.x - p.entry_blocks) * 8 + warp_id(); r < p.rows; r += step) {
+      const bool none = __ldg(p.lse2 + r) == INFINITY;
+      const int64_t at = int64_t(r) * p.words;
+#pragma unroll 4
+      for (int i = lane_id(); i < p.words; i += 32)
+        p.copy[at + i] = none ? make_uint4(0u, 0u, 0u, 0u) : __ldg(p.hidden + at + i);
+    }
+    return;
+  }
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int id = tid[i];
+  if (i >= p.n) return;
+  const int id = p.tid[i];
   if (id == kNone) return;
-  const uint32_t row = i / top;
-  const float q = fast_exp2(fmaf(zt[i], zscale, -lse2[row]));
-  dz[int64_t(row) * ld + id] = from_f32<T>((q - tp[i]) * up);
+  const uint32_t row = i / p.top;
+  const float q = fast_exp2(fmaf(p.zt[i], p.zscale, -p.lse2[row]));
+  static_cast<T*>(p.dz)[int64_t(row) * p.ld + id] = from_f32<T>((q - p.tp[i]) * p.up);
 }
 
 // out = sum over splits of part (fixed order), cast to out's dtype; 4 columns a thread.
@@ -689,7 +735,7 @@ struct BwdPlan {
   int64_t rows;        // rows per chunk
   int chunks, h_splits, h_last, w_splits;
   int64_t h_pad, w_pad;  // rows of one split's partials
-  int64_t off_dz, off_h, off_w, bytes;
+  int64_t off_dz, off_copy, off_h, off_w, bytes;
 };
 BwdPlan plan_bwd(int64_t N, int64_t V, int64_t K) {
   BwdPlan pl;
@@ -716,6 +762,7 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t K) {
     return o;
   };
   pl.off_dz = take(pl.rows * pl.ld * 2);
+  pl.off_copy = take(pl.rows * K * 2);
   const int64_t last_pad = (last + 255) / 256 * 256;
   pl.off_h = take(std::max(pl.h_splits > 1 ? pl.h_splits * pl.h_pad : 0,
                            pl.h_last > 1 ? pl.h_last * last_pad : 0) * K * 4);
@@ -738,12 +785,12 @@ int sum_splits(const float* part, int splits, int64_t split_elems, int64_t n, vo
   return check_launch("distill_bwd_sum");
 }
 
-// A gradient product's launch with `dtype` outputs of rows x K.
-template <class C, typename TO>
+// A gradient product's launch with `dtype` outputs of rows x K; `live` for dW.
+template <class C, typename TO, bool DW>
 int grad_product(const CUtensorMap& a, const CUtensorMap& b, int64_t rows, int64_t K, int64_t k_elems, int splits,
                  int64_t split_rows, void* out, int dtype, bool add, const float* inv_rows, const float* grad_out,
-                 float factor, uint32_t* status, const char* name, cudaStream_t s) {
-  TileParams<GradEpilogue<TO>> prm;
+                 float factor, const LiveHidden* live, uint32_t* status, const char* name, cudaStream_t s) {
+  TileParams<GradEpilogue<TO, DW>> prm;
   prm.tm_a = a;
   prm.tm_b = b;
   const int64_t map_rows = splits > 1 ? splits * split_rows : rows;
@@ -761,22 +808,27 @@ int grad_product(const CUtensorMap& a, const CUtensorMap& b, int64_t rows, int64
   prm.out = out;
   prm.ld_out = K;
   prm.status = status;
-  prm.ep = GradEpilogue<TO>{inv_rows, grad_out, factor, add, false};
+  prm.ep.inv_rows = inv_rows;
+  prm.ep.grad_out = grad_out;
+  prm.ep.factor = factor;
+  prm.ep.add = add;
+  prm.ep.direct = false;
+  if constexpr (DW) prm.ep.hidden = *live;
   return launch_tile_gemm<C>(prm, splits, name, s);
 }
 
-template <class C>
+template <class C, bool DW>
 int grad_product_as(int dtype, const CUtensorMap& a, const CUtensorMap& b, int64_t rows, int64_t K, int64_t k_elems,
                     int splits, int64_t split_rows, void* out, bool add, const float* inv_rows, const float* grad_out,
-                    float factor, uint32_t* status, const char* name, cudaStream_t s) {
+                    float factor, const LiveHidden* live, uint32_t* status, const char* name, cudaStream_t s) {
   if (dtype == MT_F32)
-    return grad_product<C, float>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows, grad_out,
-                                  factor, status, name, s);
+    return grad_product<C, float, DW>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows, grad_out,
+                                      factor, live, status, name, s);
   if (dtype == MT_BF16)
-    return grad_product<C, __nv_bfloat16>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows,
-                                          grad_out, factor, status, name, s);
-  return grad_product<C, __half>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows, grad_out,
-                                 factor, status, name, s);
+    return grad_product<C, __nv_bfloat16, DW>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows,
+                                              grad_out, factor, live, status, name, s);
+  return grad_product<C, __half, DW>(a, b, rows, K, k_elems, splits, split_rows, out, dtype, add, inv_rows, grad_out,
+                                     factor, live, status, name, s);
 }
 
 template <typename TL>
@@ -818,7 +870,7 @@ struct BwdArgs {
   int top;
   float temp;
   const int* tid;
-  const float *tp, *zt, *lse2, *inv_rows, *grad_out;
+  const float *tp, *zt, *lse2, *live_rows, *inv_rows, *grad_out;
   void* dh;
   int dh_dtype;
   void* dw;
@@ -837,10 +889,13 @@ int run_bwd(const BwdArgs& a, const BwdPlan& pl) {
   const float log2_up = KIND == kKindF16 ? 15.f : 0.f, up = KIND == kKindF16 ? 32768.f : 1.f;
   const float factor = a.temp / up;
   T* dz = reinterpret_cast<T*>(a.ws + pl.off_dz);
+  T* h_copy = reinterpret_cast<T*>(a.ws + pl.off_copy);
   float* h_part = reinterpret_cast<float*>(a.ws + pl.off_h);
   float* w_part = reinterpret_cast<float*>(a.ws + pl.off_w);
   // dW goes straight to its place when one fp32 tensor or one chunk takes it
   const bool w_direct = pl.w_splits == 1 && (a.dw_dtype == MT_F32 || pl.chunks == 1);
+  // live rows are counted in fp32, exact up to 2^24: past that the copy is always made
+  const float all_rows = a.N <= (1 << 24) ? float(a.N) : INFINITY;
   int st;
   for (int c = 0; c < pl.chunks; ++c) {
     const int64_t r0 = c * pl.rows, rows = std::min(pl.rows, a.N - r0);
@@ -864,9 +919,13 @@ int run_bwd(const BwdArgs& a, const BwdPlan& pl) {
     if ((st = launch_tile_gemm<Z>(zp, 1, "distill_bwd_dz", a.s)) != MT_OK) return st;
     // 2. q - p where the teacher lists an entry
     const int64_t n = rows * a.top;
-    distill_listed_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, a.s>>>(
-        a.tid + r0 * a.top, a.tp + r0 * a.top, a.zt + r0 * a.top, a.lse2 + r0, (uint32_t)n, (uint32_t)a.top, zscale, up, dz,
-        pl.ld);
+    const ListedParams lp{a.tid + r0 * a.top, a.tp + r0 * a.top, a.zt + r0 * a.top, a.lse2 + r0, (uint32_t)n,
+                          (uint32_t)a.top, (unsigned)((n + 255) / 256), zscale, up, dz, pl.ld,
+                          reinterpret_cast<const uint4*>(h), reinterpret_cast<uint4*>(h_copy), (int)rows,
+                          (int)(a.K / 8), a.live_rows, all_rows};
+    const unsigned copy_blocks =
+        a.dw != nullptr ? (unsigned)std::min<int64_t>((rows + 7) / 8, int64_t(get_sm_count()) * 8) : 0u;
+    distill_listed_kernel<T><<<lp.entry_blocks + copy_blocks, 256, 0, a.s>>>(lp);
     if ((st = check_launch("distill_bwd_listed")) != MT_OK) return st;
     // 3. dh = dz W
     if (a.dh != nullptr) {
@@ -877,12 +936,12 @@ int run_bwd(const BwdArgs& a, const BwdPlan& pl) {
       const int splits = c + 1 == pl.chunks ? pl.h_last : pl.h_splits;
       if (splits > 1) {
         const int64_t pad = (rows + 255) / 256 * 256;
-        if ((st = grad_product_as<H>(MT_F32, ma, mb, rows, a.K, a.V, splits, pad, h_part, false, a.inv_rows,
-                                     a.grad_out, factor, a.status, "distill_bwd_dh", a.s)) != MT_OK)
+        if ((st = grad_product_as<H, false>(MT_F32, ma, mb, rows, a.K, a.V, splits, pad, h_part, false, a.inv_rows,
+                                            a.grad_out, factor, nullptr, a.status, "distill_bwd_dh", a.s)) != MT_OK)
           return st;
         if ((st = sum_splits(h_part, splits, pad * a.K, rows * a.K, out, a.dh_dtype, a.s)) != MT_OK) return st;
-      } else if ((st = grad_product_as<H>(a.dh_dtype, ma, mb, rows, a.K, a.V, 1, 0, out, false, a.inv_rows,
-                                          a.grad_out, factor, a.status, "distill_bwd_dh", a.s)) != MT_OK) {
+      } else if ((st = grad_product_as<H, false>(a.dh_dtype, ma, mb, rows, a.K, a.V, 1, 0, out, false, a.inv_rows,
+                                                 a.grad_out, factor, nullptr, a.status, "distill_bwd_dh", a.s)) != MT_OK) {
         return st;
       }
     }
@@ -891,9 +950,11 @@ int run_bwd(const BwdArgs& a, const BwdPlan& pl) {
       CUtensorMap ma, mb;
       if ((st = tile_operand_map<W>(&ma, dz, true, a.V, rows, pl.ld, 0)) != MT_OK) return st;
       if ((st = tile_operand_map<W>(&mb, h, true, a.K, rows, a.K, 0)) != MT_OK) return st;
-      if ((st = grad_product_as<W>(w_direct ? a.dw_dtype : MT_F32, ma, mb, a.V, a.K, rows, pl.w_splits, pl.w_pad,
-                                   w_direct ? a.dw : w_part, c > 0, a.inv_rows, a.grad_out, factor, a.status,
-                                   "distill_bwd_dw", a.s)) != MT_OK)
+      LiveHidden live{{}, a.live_rows, all_rows};
+      if ((st = tile_operand_map<W>(&live.copy, h_copy, true, a.K, rows, a.K, 0)) != MT_OK) return st;
+      if ((st = grad_product_as<W, true>(w_direct ? a.dw_dtype : MT_F32, ma, mb, a.V, a.K, rows, pl.w_splits, pl.w_pad,
+                                         w_direct ? a.dw : w_part, c > 0, a.inv_rows, a.grad_out, factor, &live,
+                                         a.status, "distill_bwd_dw", a.s)) != MT_OK)
         return st;
     }
   }
@@ -1059,7 +1120,7 @@ extern "C" int mt_distill_bwd(const void* hidden, const void* weight, int dtype,
   if ((st = bind_device_of(hidden)) != MT_OK) return st;
   if ((st = check_arch()) != MT_OK) return st;
   const BwdArgs a{hidden, weight, N, V, K, (int)top, temperature, list_ids, list_probs, list_logits, row_stats,
-                  row_stats + N + 2, grad_out, dhidden, dh_dtype, dweight, dw_dtype, static_cast<char*>(workspace),
+                  row_stats + N + 1, row_stats + N + 2, grad_out, dhidden, dh_dtype, dweight, dw_dtype, static_cast<char*>(workspace),
                   status, s};
   if (few) return dtype == MT_BF16 ? run_few<__nv_bfloat16>(a) : run_few<__half>(a);
   return dtype == MT_BF16 ? run_bwd<__nv_bfloat16, kKindBf16>(a, pl) : run_bwd<__half, kKindF16>(a, pl);

@@ -26,6 +26,7 @@ struct Int8Epilogue {
   static constexpr uint32_t kKernelId = mt::kKernelId;
   static constexpr int OUT_SIZE = sizeof(TO);
   static constexpr bool kStats = false;
+  static constexpr bool kAltB = false;
   const float* xs;
   const float* ws;
   int n;

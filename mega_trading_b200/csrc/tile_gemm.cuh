@@ -174,6 +174,8 @@ __device__ __forceinline__ void tma_out(const CUtensorMap* map, const void* src,
 //       32 accumulator columns and their column values (shared memory) -> 16
 //       (OUT_SIZE 2) or 32 (4) packed words
 //   bool add, direct                        TMA add instead of store; plain stores
+//   static constexpr bool kAltB;            whether B may come from another tensor:
+//   const CUtensorMap* b_map(const CUtensorMap*) const    decides (device memory may say)
 // or, with `static constexpr bool kStats = true` (per_unit > 0), nothing is
 // written per tile and a thread keeps its row's state over consecutive tiles:
 //   struct State;
@@ -259,8 +261,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
   if (warp == C::EW) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
+      const CUtensorMap* tm_b = &p.tm_b;
+      if constexpr (EP::kAltB) tm_b = p.ep.b_map(tm_b);
       tma_prefetch_desc(&p.tm_a);
-      tma_prefetch_desc(&p.tm_b);
+      tma_prefetch_desc(tm_b);
       int it = 0;
       bool ok = true;
       for (int t = t_begin; ok && t < t_end; t += t_step) {
@@ -291,9 +295,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) tile_gemm_kernel(const __grid_
           }
           if constexpr (C::B_MN) {
 #pragma unroll
-            for (int j = 0; j < C::B_ROWS / 64; ++j) load(sb + j * 8192, &p.tm_b, b0 + j * 64, k);
+            for (int j = 0; j < C::B_ROWS / 64; ++j) load(sb + j * 8192, tm_b, b0 + j * 64, k);
           } else {
-            load(sb, &p.tm_b, k, b0);
+            load(sb, tm_b, k, b0);
           }
         }
       }

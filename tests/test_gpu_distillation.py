@@ -434,3 +434,27 @@ def test_distillation_entries_of_no_probability_leave_the_loss(cuda_device):
     ref = _definition(h.double(), w.double(), ids, logits, 1.0)[0]
     # the module's bound; |h| |w| <= 12 for the finite rows
     assert abs(float(loss) - float(ref)) <= 2 * (64 / 16 + 4) * 2.0 ** -23 * 12 + 1e-4
+
+
+@pytest.mark.parametrize("n,k,dtype,wdt", [
+    (2, 64, BF16, BF16),       # without tiles
+    (3, 64, BF16, BF16),
+    (140, 2056, F16, F16),
+    (6500, 768, BF16, BF16),   # two chunks of rows, the empty rows in both
+    (6500, 768, BF16, F32),    # the same into an fp32 gradient
+    (20000, 40, F16, F16),
+])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_distillation_empty_rows_may_hold_anything(cuda_device, n, k, dtype, wdt, bad):
+    """Rows without an entry, and with -inf for every listed logit, add to no gradient whatever
+    their hidden states hold: the same bits as with zeros there."""
+    g = torch.Generator(device=cuda_device).manual_seed(15)
+    h = torch.randn(n, k, device=cuda_device, generator=g).to(dtype)
+    w = (torch.randn(700, k, device=cuda_device, generator=g) * 0.1).to(wdt)
+    ids, logits = _teacher(n, 700, 6, 15, cuda_device)
+    ids[n // 2], logits[n - 1] = IGN, -float("inf")
+    h[[n // 2, n - 1]] = 0
+    want = _run(cuda_device, h, w, ids, logits, 2.0, dtype)
+    h[[n // 2, n - 1]] = bad
+    got = _run(cuda_device, h, w, ids, logits, 2.0, dtype)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
