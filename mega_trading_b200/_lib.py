@@ -13,6 +13,7 @@ import time
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libmtb200.so"
 
@@ -326,6 +327,13 @@ def require_one_device(op: str, first: torch.Tensor, *others: torch.Tensor) -> N
     for t in others:
         if t.get_device() != idx:
             raise RuntimeError(f"{op} requires all tensors on one device, found {first.device} and {t.device}")
+
+
+def has_tangent(*tensors: torch.Tensor) -> bool:
+    """Whether one of the tensors carries a forward-mode tangent."""
+    if forward_ad._current_level < 0:  # outside of any dual_level()
+        return False
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def refuse_second_derivative(op: str) -> None:

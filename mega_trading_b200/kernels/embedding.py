@@ -41,13 +41,19 @@ class _ScaledEmbedding(torch.autograd.Function):
     def forward(ctx, weight, ids, scale, padding_idx, out_dtype):
         ids, out = _lookup(weight, ids, scale, out_dtype)
         ctx.save_for_backward(ids)
-        ctx.args = (scale, padding_idx, *weight.shape, weight.dtype)
+        ctx.save_for_forward(ids)
+        ctx.args, ctx.out_dtype = (scale, padding_idx, *weight.shape, weight.dtype), out_dtype
         return out
+
+    @staticmethod
+    def jvp(ctx, weight_tangent, *_):
+        (ids,) = ctx.saved_tensors
+        return scaled_embedding(ids, weight_tangent, scale=ctx.args[0], out_dtype=ctx.out_dtype)
 
     @staticmethod
     def backward(ctx, grad_output):
         (ids,) = ctx.saved_tensors
-        if torch.is_grad_enabled() and grad_output.requires_grad:
+        if torch.is_grad_enabled() and grad_output.requires_grad or _lib.has_tangent(grad_output):
             return _EmbeddingGradient.apply(grad_output, ids, ctx.args), None, None, None, None
         return _gradient(grad_output, ids, *ctx.args), None, None, None, None
 
@@ -73,14 +79,19 @@ def _gradient(grad_output, ids, scale, padding_idx, vocab, dim, dtype):
 
 
 class _EmbeddingGradient(torch.autograd.Function):
-    """The gradient as a (linear) function of the output's gradient, for ``create_graph=True``:
-    its own gradient is the lookup again, with the padded places left out."""
+    """The gradient as a (linear) function of the output's gradient, for ``create_graph=True`` and
+    forward-mode tangents: its own gradient is the lookup again, with the padded places left out."""
 
     @staticmethod
     def forward(ctx, grad_output, ids, args):
         ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
         ctx.args, ctx.dtype = args, grad_output.dtype
         return _gradient(grad_output, ids, *args)
+
+    @staticmethod
+    def jvp(ctx, grad_tangent, *_):
+        return _gradient(grad_tangent, ctx.saved_tensors[0], *ctx.args)
 
     @staticmethod
     def backward(ctx, grad_table):
@@ -94,7 +105,8 @@ class _EmbeddingGradient(torch.autograd.Function):
 
 def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: int | None = None,
                      out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``scale * weight[ids]`` in ``out_dtype`` (the weight's by default), differentiable in ``weight``.
+    """``scale * weight[ids]`` in ``out_dtype`` (the weight's by default), differentiable in ``weight``
+    (any order, forward mode too).
 
     ``ids``: int32 or int64 of any shape; ``weight``: [vocab, dim] fp32, bf16 or fp16; the result has
     shape ``[*ids.shape, dim]``.  Places holding ``padding_idx`` (which may count from the end) look up
@@ -114,6 +126,6 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 
             raise ValueError("padding_idx must be within the vocabulary")
         pad = int(padding_idx) % weight.shape[0]
     _lib.require_one_device(op, weight, ids)
-    if not (weight.requires_grad and torch.is_grad_enabled()):
+    if not (weight.requires_grad and torch.is_grad_enabled() or _lib.has_tangent(weight)):
         return _lookup(weight, ids, float(scale), out_dtype)[1]
     return _ScaledEmbedding.apply(weight, ids, float(scale), pad, out_dtype)

@@ -299,3 +299,31 @@ def test_embedding_gradient_with_ranges_of_padding_only(cuda_device, n, dim, ot,
     for _ in range(8):
         (again,) = torch.autograd.grad(scaled_embedding(ids, w, padding_idx=pad), w, grad)
         assert torch.equal(again, first)
+
+
+@pytest.mark.parametrize("n", [5, 900])
+def test_embedding_carries_forward_mode_tangents(cuda_device, n):
+    """Tangents of the table (a parameter, a plain tensor, under no_grad) and of the output's gradient."""
+    import torch.autograd.forward_ad as fw
+
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    g = torch.Generator(device=cuda_device).manual_seed(n)
+    ids = torch.randint(0, 10, (n,), device=cuda_device, generator=g)
+    w = torch.randn(10, 8, device=cuda_device, generator=g)
+    t = torch.randn(10, 8, device=cuda_device, generator=g)
+    with fw.dual_level():
+        for leaf, grad_mode in ((w, True), (w, False), (w.clone().requires_grad_(), True),
+                                (w.clone().requires_grad_(), False)):
+            with torch.set_grad_enabled(grad_mode):
+                y = scaled_embedding(ids, fw.make_dual(leaf, t), scale=2.0, padding_idx=3, out_dtype=BF16)
+            value, tangent = fw.unpack_dual(y)
+            assert torch.equal(value.detach(), (2.0 * w[ids]).to(BF16))
+            assert torch.equal(tangent.detach(), (2.0 * t[ids]).to(BF16))
+        # forward over reverse: the gradient of sum(y^2) / 2 has the tangent of y's own gradient
+        leaf = w.clone().requires_grad_()
+        (dw,) = torch.autograd.grad(scaled_embedding(ids, fw.make_dual(leaf, t), padding_idx=3).square().sum() / 2,
+                                    leaf)
+        value, tangent = fw.unpack_dual(dw)
+        _check_grad(value, ids, w[ids], 10, 1.0, 3)
+        _check_grad(tangent, ids, t[ids], 10, 1.0, 3)
