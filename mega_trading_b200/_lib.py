@@ -336,6 +336,12 @@ def has_tangent(*tensors: torch.Tensor) -> bool:
     return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+def refuse_tangent(op: str, *tensors: torch.Tensor) -> None:
+    """For operators without a forward-mode derivative, which would return constants."""
+    if has_tangent(*tensors):
+        raise RuntimeError(f"{op} has no forward-mode gradient; call it without tangents")
+
+
 def refuse_second_derivative(op: str) -> None:
     """For backward functions whose kernels build no graph: inside ``backward(create_graph=True)``
     (the only time gradients are recorded there) raise instead of returning constants."""

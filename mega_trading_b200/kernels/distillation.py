@@ -62,6 +62,7 @@ class _FusedLinearDistillation(torch.autograd.Function):
         lib = _lib.load()
         op = "fused_linear_distillation"
         _lib.refuse_second_derivative(op)
+        _lib.refuse_tangent(op, grad_output)
         h, w, kept = ctx.saved_tensors
         temperature, top, h_dtype, w_dtype = ctx.args
         n, k = h.shape

@@ -30,10 +30,11 @@ MAX_K = 131056       # longest exact int32 dot product of 8-bit values (a multip
 
 
 def _check(op: str, first: torch.Tensor, *others: torch.Tensor) -> None:
-    """One CUDA device for all tensors, and no gradient asked of a forward-only operator."""
+    """One CUDA device for all tensors, and no gradient (of either mode) asked of a forward-only operator."""
     _lib.require_one_device(op, first, *others)
     if torch.is_grad_enabled() and (first.requires_grad or any(t.requires_grad for t in others)):
         raise RuntimeError(f"{op} has no gradient; call it under torch.no_grad()")
+    _lib.refuse_tangent(op, first, *others)
 
 
 def _rows(op: str, x: torch.Tensor) -> tuple[int, int]:

@@ -458,3 +458,24 @@ def test_distillation_empty_rows_may_hold_anything(cuda_device, n, k, dtype, wdt
     h[[n // 2, n - 1]] = bad
     got = _run(cuda_device, h, w, ids, logits, 2.0, dtype)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_distillation_refuses_forward_mode_tangents(cuda_device):
+    import torch.autograd.forward_ad as fw
+
+    from mega_trading_b200.kernels.distillation import fused_linear_distillation
+
+    g = torch.Generator(device=cuda_device).manual_seed(16)
+    h = torch.randn(4, 16, device=cuda_device, generator=g)
+    w = torch.randn(20, 16, device=cuda_device, generator=g)
+    ids, logits = _teacher(4, 20, 2, 16, cuda_device)
+    with fw.dual_level():
+        for at in range(3):
+            args = [h, w, logits]
+            args[at] = fw.make_dual(args[at], torch.ones_like(args[at]))
+            with pytest.raises(RuntimeError, match="forward mode"):  # NotImplementedError is one
+                fused_linear_distillation(args[0], args[1], ids, args[2])
+        hd = h.clone().requires_grad_()
+        loss = fused_linear_distillation(hd, w, ids, logits)
+        with pytest.raises(RuntimeError, match="no forward-mode gradient"):
+            torch.autograd.grad(loss, hd, fw.make_dual(torch.ones_like(loss), torch.ones_like(loss)))

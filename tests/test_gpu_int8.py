@@ -285,3 +285,21 @@ def test_int8_nan_scale_reaches_the_product(cuda_device):
         keep = torch.ones(rows, dtype=torch.bool, device=cuda_device)
         keep[[1, 3]] = False
         assert bool(y[keep].isfinite().all())
+
+
+def test_int8_operators_refuse_forward_mode_tangents(cuda_device):
+    import torch.autograd.forward_ad as fw
+
+    from mega_trading_b200.kernels import int8
+
+    x, w = torch.randn(4, 16, device=cuda_device), torch.ones(16, device=cuda_device)
+    q, s = int8.quantize_rows_int8(x)
+    with fw.dual_level(), torch.no_grad():
+        xd, wd, sd = (fw.make_dual(t, torch.ones_like(t)) for t in (x, w, s))
+        for call in (lambda: int8.quantize_rows_int8(xd), lambda: int8.rms_norm_int8(xd, w, eps=1e-5),
+                     lambda: int8.rms_norm_int8(x, wd, eps=1e-5),
+                     lambda: int8.add_rms_norm_int8(x, xd, w, eps=1e-5),
+                     lambda: int8.int8_linear(q, sd, q, s), lambda: int8.int8_linear(q, s, q, sd)):
+            with pytest.raises(RuntimeError, match="no forward-mode gradient"):
+                call()
+        assert torch.equal(int8.quantize_rows_int8(x)[0], q)  # without a tangent nothing is refused
