@@ -99,7 +99,7 @@ class _EmbeddingGradient(torch.autograd.Function):
         scale, padding_idx = ctx.args[:2]
         out = scaled_embedding(ids, grad_table, scale=scale, out_dtype=ctx.dtype)
         if padding_idx >= 0:
-            out = out * (ids != padding_idx).unsqueeze(-1)
+            out = out.masked_fill((ids == padding_idx).unsqueeze(-1), 0.0)  # whatever the padding row holds
         return out, None, None
 
 

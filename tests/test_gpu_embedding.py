@@ -327,3 +327,19 @@ def test_embedding_carries_forward_mode_tangents(cuda_device, n):
         value, tangent = fw.unpack_dual(dw)
         _check_grad(value, ids, w[ids], 10, 1.0, 3)
         _check_grad(tangent, ids, t[ids], 10, 1.0, 3)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_embedding_second_derivative_leaves_the_padding_row_out(cuda_device, bad):
+    """Padded places add to no gradient, so the direction's padding row reaches nothing, whatever it holds."""
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    gen = torch.Generator(device=cuda_device).manual_seed(2)
+    ids = torch.tensor([1, 2, 1, 5, 9], device=cuda_device)
+    w = torch.randn(10, 8, device=cuda_device, generator=gen, requires_grad=True)
+    g = torch.randn(5, 8, device=cuda_device, generator=gen, requires_grad=True)
+    u = torch.randn(10, 8, device=cuda_device, generator=gen)
+    u[9] = bad
+    (dw,) = torch.autograd.grad(scaled_embedding(ids, w, padding_idx=9), w, g, create_graph=True)
+    (dg,) = torch.autograd.grad(dw, g, u)
+    assert bool((dg[4] == 0).all()) and torch.equal(dg[:4], u[ids[:4]])
