@@ -103,13 +103,16 @@ class RMSNorm(nn.Module):
 
 
 class TokenEmbedding(nn.Embedding):
-    """The token table; lookup and sorted-token gradient by ``kernels.embedding`` (torch's own
-    lookup while the table is on the host)."""
+    """The token table; lookup and sorted-token gradient by ``kernels.embedding``.  Torch's own lookup
+    while the table is on the host, and for what those kernels have no form of: ``max_norm``,
+    ``sparse``, ``scale_grad_by_freq`` and tables that are not fp32, bf16 or fp16."""
 
     def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
-        if not self.weight.is_cuda:
+        w = self.weight
+        if not w.is_cuda or self.max_norm is not None or self.sparse or self.scale_grad_by_freq \
+                or w.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             return super().forward(input_ids)
-        return scaled_embedding(input_ids, self.weight, padding_idx=self.padding_idx)
+        return scaled_embedding(input_ids, w, padding_idx=self.padding_idx)
 
 
 class LlamaAttention(nn.Module):

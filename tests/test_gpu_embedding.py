@@ -343,3 +343,23 @@ def test_embedding_second_derivative_leaves_the_padding_row_out(cuda_device, bad
     (dw,) = torch.autograd.grad(scaled_embedding(ids, w, padding_idx=9), w, g, create_graph=True)
     (dg,) = torch.autograd.grad(dw, g, u)
     assert bool((dg[4] == 0).all()) and torch.equal(dg[:4], u[ids[:4]])
+
+
+@pytest.mark.parametrize("options", [dict(max_norm=0.5), dict(max_norm=1.0, norm_type=1.0), dict(sparse=True),
+                                     dict(scale_grad_by_freq=True), dict(dtype=torch.float64), dict(padding_idx=2), {}])
+def test_token_table_keeps_the_options_it_inherits(cuda_device, options):
+    from mega_trading_b200.model import TokenEmbedding
+
+    torch.manual_seed(0)
+    ours = TokenEmbedding(20, 8, device=cuda_device, **options)
+    plain = torch.nn.Embedding(20, 8, device=cuda_device, **options)
+    plain.load_state_dict(ours.state_dict())
+    ids = torch.tensor([[1, 2, 2], [3, 1, 2]], device=cuda_device)
+    out = [m(ids) for m in (ours, plain)]
+    for y in out:
+        (y.square().sum() / 4).backward()  # every product and sum of three terms is within a rounding or two
+    a, b = ours.weight.grad, plain.weight.grad
+    assert torch.equal(out[0], out[1]) and torch.equal(ours.weight, plain.weight)
+    assert a.is_sparse == b.is_sparse and a.dtype == b.dtype
+    tol = 4 * torch.finfo(a.dtype).eps * b.to_dense().abs().max()
+    assert bool(((a.to_dense() - b.to_dense()).abs() <= tol).all())
