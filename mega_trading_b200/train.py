@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import contextlib
 import datetime
+import math
 import os
 import time
 
@@ -155,12 +156,19 @@ class Trainer:
     def distill_step(self, input_ids: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
                      temperature: float = 1.0) -> torch.Tensor:
         """One optimizer step against a teacher's top logits (``[B, T, top]`` ids and logits, e.g. from
-        ``Int8TradingModel.top_logits``) instead of labels; returns the mean distillation loss."""
+        ``Int8TradingModel.top_logits``) instead of labels; returns the mean distillation loss of this
+        rank's positions that have an entry (ids of -100 mask one), however they are spread over the
+        micro-batches.  Every rank's mean counts the same, as in :meth:`step`."""
+        # positions of each sequence that the loss counts (all on the device: no host synchronisation)
+        listed = ((teacher_ids != -100) & (teacher_logits != -math.inf)).any(-1).flatten(1).sum(1)
+        total = listed.sum().clamp(min=1)
         return self._step(input_ids, lambda lo, hi: self.engine(
-            input_ids[lo:hi], teacher=(teacher_ids[lo:hi], teacher_logits[lo:hi]), temperature=temperature))
+            input_ids[lo:hi], teacher=(teacher_ids[lo:hi], teacher_logits[lo:hi]), temperature=temperature),
+            lambda lo, hi: listed[lo:hi].sum() / total)
 
-    def _step(self, input_ids: torch.Tensor, loss_of) -> torch.Tensor:
-        """One optimizer step; ``loss_of(lo, hi)`` is the engine's mean loss of a micro-batch."""
+    def _step(self, input_ids: torch.Tensor, loss_of, share_of=None) -> torch.Tensor:
+        """One optimizer step; ``loss_of(lo, hi)`` is the engine's mean loss of a micro-batch and
+        ``share_of(lo, hi)`` its weight in the batch's mean (by default its share of the sequences)."""
         if self._store is not None:
             self._await_peers()
         self._steps += 1
@@ -172,7 +180,7 @@ class Trainer:
         for i in range(chunks):
             lo = i * self.micro_batch
             hi = min(n, lo + self.micro_batch)
-            frac = (hi - lo) / n
+            frac = (hi - lo) / n if share_of is None else share_of(lo, hi)
             sync_ctx = self.engine.no_sync() if (self.world > 1 and i < chunks - 1) else contextlib.nullcontext()
             with sync_ctx:
                 loss = loss_of(lo, hi)

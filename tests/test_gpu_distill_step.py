@@ -124,3 +124,24 @@ def test_int8_model_refuses_odd_widths(cuda_device):
         q(torch.zeros(1, 513, dtype=torch.long, device=cuda_device))
     with pytest.raises(ValueError, match="shape"):
         q(torch.zeros(5, dtype=torch.long, device=cuda_device))
+
+
+def test_distill_step_of_a_padded_batch_is_the_batch_mean(cuda_device):
+    """Padding spread unevenly over the micro-batches: the loss is that of the whole batch in one piece."""
+    from mega_trading_b200.data import composite_tokens
+    from mega_trading_b200.int8_model import Int8TradingModel
+    from mega_trading_b200.model import ModelConfig
+    from mega_trading_b200.train import Trainer
+
+    teacher = Int8TradingModel(_model(cuda_device, 1, **TEACHER))
+    tr = Trainer(ModelConfig(**STUDENT), micro_batch=2, device=cuda_device, lr=1e-3)
+    ids = composite_tokens(5, 96, seed=6, device=cuda_device)
+    t_ids, t_logits = teacher.top_logits(ids, 8)
+    t_ids[0, 10:], t_ids[1, 30:], t_ids[4] = -100, -100, -100
+    t_logits[2, :40] = -float("inf")
+    with torch.no_grad():
+        want = tr.model.forward_with_distillation(ids, t_ids, t_logits, temperature=1.5)
+    got = tr.distill_step(ids, t_ids, t_logits, temperature=1.5)
+    # fp32 means of the same rows' losses
+    assert abs(float(got) - float(want)) <= 1e-5 * abs(float(want))
+    tr.check_status()
