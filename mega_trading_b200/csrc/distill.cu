@@ -728,7 +728,9 @@ int choose_k_splits(int64_t tiles, int64_t k_stages) {
   return even_splits(k_stages, best);
 }
 
-constexpr int64_t kDzBytes = int64_t(256) << 20;  // most of the workspace: one chunk's dz
+// One chunk's dz takes at most this (256 rows, the fewest of a chunk, take more
+// from a vocabulary of 524,288 on).
+constexpr int64_t kDzBytes = int64_t(256) << 20;
 
 struct BwdPlan {
   int64_t ld;          // dz row stride (elements)
@@ -766,8 +768,9 @@ BwdPlan plan_bwd(int64_t N, int64_t V, int64_t K) {
   const int64_t last_pad = (last + 255) / 256 * 256;
   pl.off_h = take(std::max(pl.h_splits > 1 ? pl.h_splits * pl.h_pad : 0,
                            pl.h_last > 1 ? pl.h_last * last_pad : 0) * K * 4);
-  // fp32 sums of dW: several splits, or several chunks of a 16-bit gradient
-  pl.off_w = take(pl.w_splits * pl.w_pad * K * 4);
+  // fp32 sums of dW: several splits, or several chunks (of a 16-bit gradient; the
+  // size does not know the type).  One split of one chunk goes straight to its place.
+  pl.off_w = take(pl.w_splits > 1 || pl.chunks > 1 ? pl.w_splits * pl.w_pad * K * 4 : 0);
   pl.bytes = at;
   return pl;
 }

@@ -147,3 +147,15 @@ def test_token_table_on_the_host_still_looks_up():
                                      kv_heads=2, intermediate_dim=48))
     ids = torch.tensor([[1, 2, 3]])
     assert torch.equal(m.token_embedding(ids), m.token_embedding.weight[ids])
+
+
+def test_distillation_workspace_holds_what_the_call_uses():
+    """No room for partial sums of dW where one product writes dW itself (one chunk of rows, one split);
+    room for them where chunks of rows add up."""
+    from mega_trading_b200 import _lib
+
+    size = _lib.load().mt_distill_bwd_workspace_bytes
+    # dz, the chunk's hidden states and at most 64 splits of dh in fp32
+    for n, v, k in ((256, 300_000, 1024), (8, 1_200_000, 1024), (200, 21_504, 256)):
+        assert size(n, v, k) <= 2 * n * (v + 8) + 2 * n * k + 64 * 256 * k * 4 + 4 * 256
+    assert size(20_000, 21_504, 768) >= 21_504 * 768 * 4
