@@ -623,13 +623,25 @@ __global__ void __launch_bounds__(kBulkThreads) embed_reduce_bulk_kernel(
     // ------------------------------------------------------------ add
     const bool own = threadIdx.x * 16 < (int)bytes;
     const int col = c0 + threadIdx.x * E;
-    float acc[E];
+    // a run's latest rows, 64 at most, and the sum of those before them: a long run
+    // carries about 64 + rows / 64 roundings instead of one per row
+    float acc[E], sum[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int e = 0; e < E; ++e) acc[e] = sum[e] = 0.f;
+    int held = 0;        // rows in acc, or more
     bool begins = true;  // the current run begins in this range
     int64_t at = lo;
     for (int it = 0; at < hi; ++it) {
       const int st = it % kBulkStages;
+      if (held + rp > 64) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          sum[e] += acc[e];
+          acc[e] = 0.f;
+        }
+        held = 0;
+      }
+      held += rp;
       if (!__all_sync(0xffffffffu, wait_bounded(wc, &sm.full[st], (it / kBulkStages) & 1, 2))) break;
       const int rows = (int)min((int64_t)rp, hi - at);
       // four rows at a time: their values and run flags are fetched together
@@ -680,6 +692,8 @@ __global__ void __launch_bounds__(kBulkThreads) embed_reduce_bulk_kernel(
           const bool ends = m[j].y & kRunEnds;
           if (ends && blockIdx.y == 0 && threadIdx.x == 0) seg[m[j].x].y = (uint32_t)here + 1u;
           if (ends || here + 1 == hi) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += sum[e];
             if (own) {
               if (begins && ends) {
 #pragma unroll
@@ -690,7 +704,7 @@ __global__ void __launch_bounds__(kBulkThreads) embed_reduce_bulk_kernel(
               }
             }
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = 0.f;
+            for (int e = 0; e < E; ++e) acc[e] = sum[e] = 0.f;
           }
         }
       }

@@ -363,3 +363,27 @@ def test_token_table_keeps_the_options_it_inherits(cuda_device, options):
     assert a.is_sparse == b.is_sparse and a.dtype == b.dtype
     tol = 4 * torch.finfo(a.dtype).eps * b.to_dense().abs().max()
     assert bool(((a.to_dense() - b.to_dense()).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("n,dim,run,ot", [
+    (262144, 64, 800, F32),
+    (262144, 96, 800, BF16),
+    (262144, 1024, 900, F32),    # four rows to a stage of the gather ring
+    (1100000, 8, 3000, F32),
+    (60000, 510, 800, F32),      # not on the bulk path: chunks of 64
+    (30000, 40, 150, F16),
+])
+def test_embedding_long_runs_keep_the_bound(cuda_device, n, dim, run, ot):
+    """Every row of a run but its first is too small to change the first's sum by itself: one rounding
+    per row would lose them all, the bound of the module docstring allows some of them."""
+    from mega_trading_b200.kernels.embedding import scaled_embedding
+
+    vocab = n // run + 1
+    ids = torch.arange(n, device=cuda_device) // run
+    big = 2.0 ** 11 if ot is F16 else 2.0 ** 24
+    grad = torch.full((n, dim), 0.875 * big * 2.0 ** -24, device=cuda_device, dtype=F32)
+    grad[::run] = big
+    grad = grad.to(ot)
+    w = torch.zeros(vocab, dim, device=cuda_device, requires_grad=True)
+    (dw,) = torch.autograd.grad(scaled_embedding(ids, w, out_dtype=ot), w, grad)
+    _check_grad(dw, ids, grad, vocab, 1.0, None)
