@@ -71,6 +71,18 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
+// Sum of squares of a row times `factor` squared, by one warp.
+template <typename T>
+__device__ __forceinline__ float scaled_squares(const T* s, int dim, float factor) {
+  float a = 0.f;
+#pragma unroll 1
+  for (int i = lane_id(); i < dim; i += 32) {
+    const float v = to_f32<T>(s[i]) * factor;
+    a = fmaf(v, v, a);
+  }
+  return warp_sum(a);
+}
+
 struct QParams {
   const void* x;
   const void* res;   // ADD
@@ -262,10 +274,6 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quant8_kernel(const __g
   // an infinity or a NaN anywhere in the row: the scale is NaN
   const bool finite = amax < INFINITY;
   const float inv = finite && amax >= kTinyAmax ? __fdiv_rn(127.f, amax) : 0.f;
-  if (t == 0) {
-    const float rs = MODE == kPlain ? 1.f : rsqrtf(ss / float(dim) + p.eps);
-    p.scale[row] = !finite ? NAN : (amax >= kTinyAmax || isnan(rs) ? amax * rs / 127.f : 0.f);
-  }
   int8_t* q = p.q + row * dim;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -282,6 +290,21 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quant8_kernel(const __g
         if (col_of(c, e) < dim) q[col_of(c, e)] = (int8_t)(b[e] & 0xFFu);
     }
   }
+  if (t >= 32) return;
+  float rs = 1.f;
+  if constexpr (MODE != kPlain) {
+    rs = rsqrtf(ss / float(dim) + p.eps);
+    // Squares outside fp32's range (values of about 2^59 and more, or below 2^-50
+    // with next to no eps): the row's first warp sums them again from memory, scaled.
+    const bool over = ss == INFINITY, under = ss < 0x1p-100f && p.eps < 0x1p-80f;
+    if (finite && amax >= kTinyAmax && (over || under)) {
+      const float f = over ? 0x1p-80f : 0x1p80f;
+      __syncwarp();  // new_res is read across the lanes that wrote it (wider rows met at the barrier above)
+      const float sq = MODE == kAddNorm ? scaled_squares<TR>(nr, dim, f) : scaled_squares<TX>(x, dim, f);
+      rs = rsqrtf(sq / float(dim) + p.eps * f * f) * f;
+    }
+  }
+  if (t == 0) p.scale[row] = !finite ? NAN : (amax >= kTinyAmax || isnan(rs) ? amax * rs / 127.f : 0.f);
 }
 
 bool al(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }

@@ -303,3 +303,36 @@ def test_int8_operators_refuse_forward_mode_tangents(cuda_device):
             with pytest.raises(RuntimeError, match="no forward-mode gradient"):
                 call()
         assert torch.equal(int8.quantize_rows_int8(x)[0], q)  # without a tangent nothing is refused
+
+
+@pytest.mark.parametrize("dim", [40, 41, 768, 1024, 1500, 5000, 9001, 32768])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_int8_of_rows_whose_squares_leave_fp32(cuda_device, dim, dtype):
+    """Rows of the type's lowest and largest values, of 1e25, one such value alone, and (without eps) of
+    1e-30: the scale is the definition's although the sum of squares is outside fp32's range."""
+    from mega_trading_b200.kernels import int8
+
+    g = torch.Generator().manual_seed(dim)
+    x = torch.randn(8, dim, generator=g)
+    x[0] = torch.finfo(dtype).min
+    x[1] = torch.finfo(dtype).max * torch.rand(dim, generator=g)
+    x[2] *= 1e25
+    x[3, dim // 2] = 3e38
+    x[4] *= 1e-30
+    x[5] *= 1e-20
+    x[6] = 0
+    x = x.to(dtype)
+    w = 0.2 + 0.5 * torch.rand(dim, generator=g)
+    r = torch.zeros(8, dim, dtype=dtype)
+    for eps in (1e-5, 0.0):
+        if eps == 0.0:
+            x[7, 0] = 1.0
+        s, q, amax = x.float(), *_quant_ref(x.float() * w)
+        want = amax.double() / 127 * (s.double().pow(2).mean(-1) + eps).rsqrt()
+        want[6] = 0.0
+        got = int8.rms_norm_int8(x.to(cuda_device), w.to(cuda_device), eps=eps)
+        new = int8.add_rms_norm_int8(x.to(cuda_device), r.to(cuda_device), w.to(cuda_device), eps=eps)
+        assert torch.equal(new[0].cpu(), x)
+        for qq, scale in (got, new[1:]):
+            assert torch.equal(qq.cpu(), q)
+            _close(scale, want, 1e-5)
