@@ -359,7 +359,8 @@ MT_API int mt_fused_ce_bwd(const void* hidden, const void* weight, const void* l
  * hidden [N, K], weight [V, K] bf16 or fp16 (dtype), contiguous, 16-byte
  * aligned, K % 8 == 0; teacher_ids [N, top] int64 (ids_i64 = 1) or int32,
  * teacher_logits [N, top] in logits_dtype, contiguous, 1 <= top <= 256, in any
- * order, ids may repeat.  An entry whose id is ignore_index is masked: its
+ * order; ids may repeat (each entry has its own term: KL(p || q) for distinct ids).
+ * An entry whose id is ignore_index is masked: its
  * logit is not used, whatever it holds.  Ids outside [0, V) are masked too and
  * set the status word ((8 << 16) | 0xEEEE).  Rows without an entry of finite
  * weight (all masked, or all logits -inf) add neither loss nor gradient; loss

@@ -5,8 +5,10 @@ Beside the fused linear + cross-entropy (``fused_ce.py``): the same projection
 largest logits of a teacher per row instead of one label.  With ``p`` the
 softmax of a row's listed teacher logits and ``q`` the student's softmax over
 the whole vocabulary, both at ``temperature``, the loss is
-``temperature**2 * mean_rows KL(p || q)`` (the factor keeps gradients comparable
-across temperatures).  The reference (duoan/mega-trading) has no distillation.
+``temperature**2 * mean_rows sum_j p_j (log p_j - log q[id_j])`` over the listed
+entries: ``KL(p || q)`` when a row's ids are distinct (the factor keeps gradients
+comparable across temperatures).  The reference (duoan/mega-trading) has no
+distillation.
 """
 
 from __future__ import annotations
@@ -94,15 +96,20 @@ def _aligned(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 def fused_linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
                               teacher_logits: torch.Tensor, *, temperature: float = 1.0, ignore_index: int = -100,
                               compute_weight: torch.Tensor | None = None) -> torch.Tensor:
-    """``temperature**2 * mean_rows KL(softmax(teacher_logits / T) || softmax(hidden @ weight.T / T))`` (fp32 scalar).
+    """``temperature**2 * mean_rows sum_j p_j (log p_j - log q[teacher_ids_j])`` (fp32 scalar) with
+    ``p = softmax(teacher_logits / T)`` and ``q = softmax(hidden @ weight.T / T)``.
 
     ``hidden`` [rows, hidden_dim] and ``weight`` [vocab, hidden_dim]; ``teacher_ids`` (int32 / int64) and
     ``teacher_logits`` (fp32 / bf16 / fp16) [rows, top], ``top`` at most 256, in any order.  The teacher's
     distribution is normalised over a row's listed entries; entries whose id is ``ignore_index`` are left
-    out (their logits may hold anything), an id listed twice counts with the sum of its probabilities.  Rows
-    without an entry (padding) add neither loss nor gradient.  A teacher id outside the vocabulary is left
-    out and sets the device status word.  Gradients go to ``hidden`` and ``weight`` in their own dtypes, not
-    to the teacher; 16-bit products with fp32 sums (an fp32 ``hidden`` or ``weight`` is rounded to bf16).
+    out (their logits may hold anything).  With distinct ids a row's sum is ``KL(p || q)``.  An id listed
+    several times counts once per entry: the gradients are those of the KL divergence from the merged list,
+    the loss is lower than it by the entropy of the split (which the student does not change) and may be
+    negative.  Rows without an entry (padding) add neither loss nor gradient, whatever their hidden states
+    hold.  A teacher id outside the vocabulary is left out and sets the device status word.  Gradients go to
+    ``hidden`` and ``weight`` in their own dtypes, not to the teacher.  Products of 16-bit operands with fp32
+    sums: in ``hidden``'s type when it is 16 bits wide, else bf16, to which the other operand is rounded; the
+    backward rounds ``q - p`` to that type once (not for one or two rows).
 
     ``compute_weight``: an optional 16-bit copy of ``weight`` that the kernels read instead of casting it,
     as in :func:`~mega_trading_b200.kernels.fused_ce.fused_linear_cross_entropy`."""

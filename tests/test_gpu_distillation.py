@@ -479,3 +479,26 @@ def test_distillation_refuses_forward_mode_tangents(cuda_device):
         loss = fused_linear_distillation(hd, w, ids, logits)
         with pytest.raises(RuntimeError, match="no forward-mode gradient"):
             torch.autograd.grad(loss, hd, fw.make_dual(torch.ones_like(loss), torch.ones_like(loss)))
+
+
+def test_distillation_of_repeated_ids_against_the_merged_list(cuda_device):
+    """Each listing of an id is an entry of its own: the gradients are those of the merged list, the loss
+    is lower by the entropy of the split."""
+    g = torch.Generator(device=cuda_device).manual_seed(17)
+    n, v, k, temp = 60, 300, 64, 1.5
+    h = torch.randn(n, k, device=cuda_device, generator=g)
+    w = torch.randn(v, k, device=cuda_device, generator=g) * 0.1
+    ids = torch.randperm(v, device=cuda_device, generator=g)[:3].expand(n, 3)
+    logits = torch.randn(n, 6, device=cuda_device, generator=g) * 2
+    split = _run(cuda_device, h, w, ids.repeat(1, 2), logits, temp, BF16)
+    merged = torch.logsumexp(logits.view(n, 2, 3).double() / temp, 1) * temp
+    whole = _run(cuda_device, h, w, ids, merged.float(), temp, BF16)
+    p, big = torch.softmax(logits.double() / temp, 1), torch.softmax(merged / temp, 1)
+    gap = temp ** 2 * float((torch.special.xlogy(big, big).sum(1) - torch.special.xlogy(p, p).sum(1)).mean())
+    assert gap > 0.1
+    # the module's bound of a loss, twice (|z| errors below 1e-5 here)
+    assert abs(float(whole[0]) - float(split[0]) - gap) <= 2 * temp ** 2 * 2e-4
+    for a, b in zip(split[1:], whole[1:]):
+        # fp32 outputs of dz rounded to bf16: a probability that lands on the other side of a rounding border
+        # moves its entry by one step, 2^-8 of it
+        assert float((a - b).abs().max()) <= 2.0 ** -7 * float(b.abs().max())
