@@ -17,7 +17,8 @@ namespace {
 
 constexpr uint32_t kKernelId = 9;
 constexpr int kMaxK = 131056;
-// us, dot products / 128 x 128 tiles: 21,504 x 768 with 4 tokens 5.1 / 8.2, 8
+// us with w in the L2 (4 tokens from a cold one: 8.8), dot products / 128 x 128
+// tiles: 21,504 x 768 with 4 tokens 5.1 / 8.2, 8
 // tokens 8.0 / 8.9, 16 tokens 13.8 / 8.8; 1,280 x 768 2.3 / 4.9, 3.2 / 4.8, 4.5 / 4.8
 constexpr int kFewTokens = 8;
 
@@ -65,8 +66,9 @@ struct Int8Epilogue {
 
 // 8 lanes per channel, 4 channels per warp, 32 channels per block; MT tokens
 // (rows past M are zero).  Blocks of 1,024 of K: a lane's 8 x 16 bytes of w are on
-// their way to registers before the tokens' part of x is staged, so all of w is
-// in flight at once (21,504 x 768: every block of the grid is resident).
+// their way to registers before the tokens' part of x is staged, so all of a
+// resident block's w is in flight at once (21,504 x 768 has 672 blocks: all of them
+// with one token, 592 with two to four, 444 with up to eight).
 template <typename TO, int MT>
 __global__ void __launch_bounds__(256) int8_few_kernel(const int8_t* __restrict__ x, const float* __restrict__ xs,
                                                        const int8_t* __restrict__ w, const float* __restrict__ ws,

@@ -12,12 +12,13 @@
 // squares was taken, and is the same integer for any grouping of threads.  A
 // row whose a is below 2^-119 (127 / a would overflow) gives q = 0, scale = 0;
 // a row with an infinity or a NaN gives a NaN scale, so whatever is computed
-// from it is NaN too (its q means nothing).
+// from it is NaN too (its q means nothing).  Squares past fp32's range are summed
+// again, scaled: a row of the type's lowest value has its scale.
 //
 // Bound by HBM: each element is read once (plus the residual read and written)
 // and leaves as one byte (131,072 x 1,024, bf16 branch and fp32 residual: 235
-// us, 0.96 of the measured copy rate; 30,011 x 2,816 bf16 without a norm: 41 us,
-// 0.94).  The row stays in registers between the reduction and the
+// us, 0.96 of the measured copy rate; 30,011 x 2,816 bf16 without a norm: 41-43
+// us, 0.91-0.95).  The row stays in registers between the reduction and the
 // quantisation.  One warp owns a row of up to 1024 elements; wider
 // rows take 128, 256 or 1024 threads (their statistics meet in shared memory).
 // Accesses are 16-byte vectors when the width and every address allow it,
