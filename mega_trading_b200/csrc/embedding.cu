@@ -158,16 +158,21 @@ constexpr int lane_elems() {
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-// TPW tokens per warp, one after the other: 4 keep the loads of 16-bit rows (1.5
-// KB and less) coming while a row is written (262,144 x 768 bf16: 74 us, 85 us
-// with one), 1 spreads few tokens or long rows over more warps.
+// TPW tokens per warp, one after the other: 4 keep the loads of 16-bit rows coming
+// while a row is written, 1 spreads few tokens over more warps.  bf16 from a cold L2,
+// us with 4 / 1: 8,000 tokens x 256 5.6 / 4.5, x 768 11.3 / 8.1; 18,944 (where 4
+// begin) x 256 6.5 / 7.0, x 768 13.5 / 12.8; 131,072 x 256 22.5 / 29.7, x 768
+// 51.5 / 54.7, x 1,024 70.1 / 70.8, x 2,048 150 / 141.  fp32 rows take 1.
 template <typename TW, typename TO, bool VEC, int TPW>
 __global__ void __launch_bounds__(256) embed_fwd_kernel(const void* __restrict__ ids, int i64, int64_t n_tokens,
                                                         const TW* __restrict__ w, int64_t vocab, int dim, float scale,
                                                         TO* __restrict__ y, uint32_t* status) {
   constexpr int E = lane_elems<TW, TO>();
   using C = Cols<E, VEC>;
-  constexpr int kSlabs = 24 / E;  // 768 columns in flight (1,024 cost 30-40 % of the 16-bit rate in occupancy)
+  // 768 columns in flight: 131,072 bf16 rows of 768 51.5 us (1,024 in flight 58.2 in
+  // occupancy, 512 48.3), of 1,024 70.1 (76.4, 62.9); 2,000 fp32 rows of 768 3.1 (3.1,
+  // 3.7), 131,072 of 1,024 112.2 (111.8, 112.8)
+  constexpr int kSlabs = 24 / E;
   const int64_t n0 = (int64_t(blockIdx.x) * 8 + warp_id()) * TPW;
   int64_t mine = 0;
   if (lane_id() < TPW && n0 + lane_id() < n_tokens) mine = load_id(ids, i64, n0 + lane_id());

@@ -17,8 +17,10 @@ namespace {
 
 constexpr uint32_t kKernelId = 9;
 constexpr int kMaxK = 131056;
-// us with w in the L2 (4 tokens from a cold one: 8.8), dot products / 128 x 128
-// tiles: 21,504 x 768 with 4 tokens 5.1 / 8.2, 8
+// us, dot products / 128 x 128 tiles.  From a cold L2, 21,504 channels: K = 768 with
+// 4 tokens 7.8 / 10.0, 8 tokens 10.2 / 10.1; K = 1,024 9.1 / 11.8, 12.3 / 11.8; K =
+// 2,816 18.0 / 25.2, 25.0 / 24.9; 1,280 channels, K = 2,816, 8 tokens 9.1 / 10.8.
+// With w in the L2: 21,504 x 768 with 4 tokens 5.1 / 8.2, 8
 // tokens 8.0 / 8.9, 16 tokens 13.8 / 8.8; 1,280 x 768 2.3 / 4.9, 3.2 / 4.8, 4.5 / 4.8
 constexpr int kFewTokens = 8;
 

@@ -333,7 +333,9 @@ int dispatch(const QParams& p, cudaStream_t s) {
   if (chunks <= 32) return launch_q<TX, TR, MODE, 32, 1>(p, vec, s);
   // Few rows: four warps per row shorten the one wave there is (8 x 1,024, norm:
   // 2.2 us, one warp 3.9); many rows want no exchange between warps (65,536 x
-  // 1,024 without a norm: 34.7 us, four warps 45.4).
+  // 1,024 without a norm: 34.7 us, four warps 45.4).  Between them, four warps / one:
+  // 592 x 512 without a norm 1.84 / 1.74 us, 592 x 1,024 with the add and the norm 3.6 /
+  // 5.7, 2,368 x 1,024 6.8 / 7.8, 4,736 x 1,024 11.7 / 11.2.
   if (chunks <= 128 && p.rows <= 4 * int64_t(get_sm_count())) return launch_q<TX, TR, MODE, 128, 1>(p, vec, s);
   if (chunks <= 64) return launch_q<TX, TR, MODE, 32, 2>(p, vec, s);
   if (chunks <= 96) return launch_q<TX, TR, MODE, 32, 3>(p, vec, s);
