@@ -169,9 +169,9 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const void* __restrict__
                                                         TO* __restrict__ y, uint32_t* status) {
   constexpr int E = lane_elems<TW, TO>();
   using C = Cols<E, VEC>;
-  // 768 columns in flight: 131,072 bf16 rows of 768 51.5 us (1,024 in flight 58.2 in
-  // occupancy, 512 48.3), of 1,024 70.1 (76.4, 62.9); 2,000 fp32 rows of 768 3.1 (3.1,
-  // 3.7), 131,072 of 1,024 112.2 (111.8, 112.8)
+  // 768 columns in flight.  us with 768 / 1,024 / 512: 131,072 bf16 rows of 768 51.5 /
+  // 58.2 / 48.3, of 1,024 70.1 / 76.4 / 62.9; 2,000 fp32 rows of 768 3.1 / 3.1 / 3.7,
+  // 131,072 of 1,024 112.2 / 111.8 / 112.8
   constexpr int kSlabs = 24 / E;
   const int64_t n0 = (int64_t(blockIdx.x) * 8 + warp_id()) * TPW;
   int64_t mine = 0;
