@@ -33,8 +33,8 @@
 // two rows take a path without tiles or that rounding.
 //
 // Bound by the tensor pipe and, in a steady stream, by the power limit: 32,768
-// rows x 768 against 21,504 entries, forward and backward, 3.70-3.81 ms (8 NVK
-// operations at 1.14-1.17 PFLOP/s).  Alone: statistics 745-759 us (tensor pipe
+// rows x 768 against 21,504 entries, forward and backward, 3.70-3.89 ms (8 NVK
+// operations at 1.11-1.17 PFLOP/s).  Alone: statistics 745-759 us (tensor pipe
 // 81-82 % busy), per 6,144-row chunk dz 148 us (82 %), dh 128-130 us (93 %), dW
 // 138-144 us (81-85 %: 252 tiles in two splits on 74 CTA pairs, 6.8 of 7 waves,
 // each chunk added to two 66 MB sets of fp32 sums).
